@@ -1,0 +1,443 @@
+// Attention with capped and biased scores under document, prefix, causal and window masks
+// (eg2_attention_masked in include/eg2.h).
+//
+//   x(i, j) = cap * tanh(scale * q_i . k_j / cap)  (or scale * q_i . k_j)  + bias(j - i)
+//   out_i   = sum_j softmax_j(x(i, j)) v_j over the keys j that i may see,  lse_i = log sum_j exp x(i, j)
+//
+// i and j are places within the sequence; the queries are its last places. What i may see is an interval
+// [lo, hi) of keys -- the window and the causal or prefix bound -- less the keys of other documents. A row that
+// sees nothing gets out = 0, lse = -inf. Keys that a row may not see contribute nothing whatever they hold.
+#include "common.cuh"
+#include "kernels.h"
+
+#include <cmath>
+#include <type_traits>
+
+namespace eg2 {
+
+struct MaskedParams {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    long ldq, ldk, ldv, ldo;
+    const int *q_off, *k_off, *prefix, *q_doc, *k_doc;
+    const float *slopes, *table;
+    long q_rows, k_rows;
+    int n_seq, max_q, max_k, nh, nkv, hd, G, window, causal, radius, nsplit;
+    float scale, softcap;
+    float *part_o, *part_lse;  // nsplit > 1: [nsplit][q_rows][nh][hd] and [nsplit][q_rows][nh]
+};
+
+// One sequence: its rows, clamped to the buffers and to the stated maxima whatever the offsets hold.
+struct MaskedSeq {
+    long q0, k0;
+    int nq, nk, prefix;
+};
+EG2_DEV MaskedSeq masked_seq(const MaskedParams& p, int b) {
+    MaskedSeq s;
+    auto bound = [](long x, long lo, long hi) { return x < lo ? lo : x > hi ? hi : x; };
+    s.q0 = bound(p.q_off[b], 0, p.q_rows);
+    s.k0 = bound(p.k_off[b], 0, p.k_rows);
+    s.nq = (int)min(bound(p.q_off[b + 1], s.q0, p.q_rows) - s.q0, (long)p.max_q);
+    s.nk = (int)min(bound(p.k_off[b + 1], s.k0, p.k_rows) - s.k0, (long)p.max_k);
+    s.prefix = p.prefix ? p.prefix[b] : 0;
+    return s;
+}
+// Keys [lo, hi) of the query at place i (before the document mask).
+EG2_DEV void masked_range(const MaskedParams& p, const MaskedSeq& s, int i, int& lo, int& hi) {
+    lo = 0;
+    hi = s.nk;
+    if (p.window >= 0) {
+        lo = max(0, i - p.window);
+        hi = min(hi, (int)min((long)i + p.window + 1, (long)s.nk));
+    }
+    if (p.causal) hi = min(hi, max(i + 1, s.prefix));
+}
+
+// ---------------------------------------------------------------------------------------------
+// CUDA cores, f32 arithmetic. A block takes 16 RPT rows (row r = token r / G, head r % G of the K/V head's G
+// query heads) and walks 64-key tiles; thread (ty, tx) holds RPT x 4 scores and RPT x 4 channels of each
+// 64-channel chunk of the output. K and V pass through shared memory in chunks of 64 keys x 64 channels, the
+// next chunk's loads in flight (in registers) while one is used.
+// ---------------------------------------------------------------------------------------------
+constexpr int AMS_LD = 68;  // floats per staged row: 16-byte units of neighbouring rows in different banks
+
+template <typename T>
+EG2_DEV float4 ams_load4(const T* p, int n, bool vec) {  // n valid elements
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (n >= 4 && vec) {
+        if constexpr (sizeof(T) == 4) {
+            r = *reinterpret_cast<const float4*>(p);
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            r = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                            __uint_as_float(u.y & 0xffff0000u));
+        }
+    } else {
+        if (n > 0) r.x = ldf(p, 0);
+        if (n > 1) r.y = ldf(p, 1);
+        if (n > 2) r.z = ldf(p, 2);
+        if (n > 3) r.w = ldf(p, 3);
+    }
+    return r;
+}
+
+template <typename T, int NCH, int RPT>
+__global__ void __launch_bounds__(256) attention_masked_simt_kernel(const MaskedParams p, int q_tiles, int vec) {
+    constexpr int TR = 16 * RPT, QLD = 64 * NCH + 4;
+    extern __shared__ float ams_smem[];
+    float* qs = ams_smem;                 // [TR][QLD]
+    float* kv = qs + TR * QLD;            // [64][AMS_LD]
+    float* ps = kv + 64 * AMS_LD;         // [TR][AMS_LD]
+    int* docs = (int*)(ps + TR * AMS_LD); // [64]
+    const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+    // Heavy tiles first: under a causal mask the last queries see the most keys.
+    long id = blockIdx.x;
+    const int g = (int)(id % p.nkv);
+    id /= p.nkv;
+    const int b = (int)(id % p.n_seq);
+    const int tile = q_tiles - 1 - (int)(id / p.n_seq);
+    const MaskedSeq sq = masked_seq(p, b);
+    const int r0 = tile * TR, n_rows = sq.nq * p.G;  // nq * G < 2^31: checked on the host
+    if (r0 >= n_rows) return;
+    const int split = blockIdx.y;
+    const T* Q = (const T*)p.q;
+    const T* K = (const T*)p.k;
+    const T* V = (const T*)p.v;
+
+    for (int i = tid; i < TR * NCH * 16; i += 256) {
+        const int r = i / (NCH * 16), c = (i % (NCH * 16)) * 4;
+        const int rr = r0 + r;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (rr < n_rows) x = ams_load4(Q + (sq.q0 + rr / p.G) * p.ldq + (long)(g * p.G + rr % p.G) * p.hd + c, p.hd - c, vec);
+        *reinterpret_cast<float4*>(qs + r * QLD + c) = x;
+    }
+    int lo[RPT], hi[RPT], place[RPT], qdoc[RPT], head[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+        const int rr = r0 + ty * RPT + i;
+        const int t = rr < n_rows ? rr / p.G : 0;
+        place[i] = sq.nk - sq.nq + t;
+        head[i] = g * p.G + rr % p.G;
+        masked_range(p, sq, place[i], lo[i], hi[i]);
+        if (rr >= n_rows) lo[i] = hi[i] = 0;
+        qdoc[i] = p.q_doc ? p.q_doc[sq.q0 + t] : 0;
+    }
+    // The union of the rows' ranges, and the documents that they belong to.
+    const int t_first = r0 / p.G, t_last = (min(n_rows, r0 + TR) - 1) / p.G;
+    int k_lo, k_hi, tmp, doc_lo = 0, doc_hi = 0;
+    masked_range(p, sq, sq.nk - sq.nq + t_first, k_lo, tmp);
+    masked_range(p, sq, sq.nk - sq.nq + t_last, tmp, k_hi);
+    if (p.q_doc) {
+        doc_lo = doc_hi = p.q_doc[sq.q0 + t_first];
+        for (int t = t_first + 1; t <= t_last; t++) {
+            const int d = p.q_doc[sq.q0 + t];
+            doc_lo = min(doc_lo, d);
+            doc_hi = max(doc_hi, d);
+        }
+    }
+    const int first = k_lo / 64, tiles = k_hi > k_lo ? (k_hi + 63) / 64 - first : 0;
+    const int j_first = first + (int)((long)tiles * split / p.nsplit), j_last = first + (int)((long)tiles * (split + 1) / p.nsplit);
+
+    float m[RPT], l[RPT], o[NCH][RPT][4];
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NCH; c++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[c][i][x] = 0.f;
+    }
+    const float inv_cap = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
+    const int lr = tid >> 4, lc = (tid & 15) * 4;  // staged element: rows lr + 16 x, channels lc ..
+    float4 st[4];
+    for (int j = j_first; j < j_last; j++) {
+        const int key0 = j * 64;
+        auto fetch = [&](const T* base, long ld, int ch) {
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int key = key0 + lr + 16 * x;
+                st[x] = key < sq.nk ? ams_load4(base + (sq.k0 + key) * ld + (long)g * p.hd + ch * 64 + lc, p.hd - ch * 64 - lc, vec)
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        auto stage = [&] {
+#pragma unroll
+            for (int x = 0; x < 4; x++) *reinterpret_cast<float4*>(kv + (lr + 16 * x) * AMS_LD + lc) = st[x];
+        };
+        __syncthreads();  // the previous tile's V and documents are done with
+        if (p.k_doc) {
+            bool hit = false;
+            if (tid < 64 && key0 + tid < sq.nk) {
+                const int d = p.k_doc[sq.k0 + key0 + tid];
+                docs[tid] = d;
+                hit = d >= doc_lo && d <= doc_hi;
+            }
+            if (!__syncthreads_or(hit)) continue;
+        }
+        fetch(K, p.ldk, 0);
+        float s[RPT][4];
+#pragma unroll
+        for (int i = 0; i < RPT; i++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) s[i][x] = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < NCH; ch++) {
+            if (ch) __syncthreads();
+            stage();
+            __syncthreads();
+            if (ch + 1 < NCH)
+                fetch(K, p.ldk, ch + 1);
+            else
+                fetch(V, p.ldv, 0);
+#pragma unroll 4
+            for (int d = 0; d < 64; d += 4) {
+                float4 a[RPT], w[4];
+#pragma unroll
+                for (int i = 0; i < RPT; i++) a[i] = *reinterpret_cast<const float4*>(qs + (ty * RPT + i) * QLD + ch * 64 + d);
+#pragma unroll
+                for (int x = 0; x < 4; x++) w[x] = *reinterpret_cast<const float4*>(kv + (tx + 16 * x) * AMS_LD + d);
+#pragma unroll
+                for (int i = 0; i < RPT; i++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        s[i][x] = fmaf(a[i].x, w[x].x, s[i][x]);
+                        s[i][x] = fmaf(a[i].y, w[x].y, s[i][x]);
+                        s[i][x] = fmaf(a[i].z, w[x].z, s[i][x]);
+                        s[i][x] = fmaf(a[i].w, w[x].w, s[i][x]);
+                    }
+            }
+        }
+        // Scores of keys key0 + tx + 16 x.
+        bool hidden = false;
+#pragma unroll
+        for (int i = 0; i < RPT; i++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int key = key0 + tx + 16 * x;
+                float v = p.softcap > 0.f ? p.softcap * tanhf(s[i][x] * inv_cap) : s[i][x] * p.scale;
+                const int apart = key - place[i];
+                if (p.slopes) v -= p.slopes[head[i]] * fabsf((float)apart);
+                if (p.table) v += p.table[(long)head[i] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)];
+                const bool seen = key >= lo[i] && key < hi[i] && (!p.k_doc || docs[tx + 16 * x] == qdoc[i]);
+                hidden |= !seen;
+                s[i][x] = seen ? v : -INFINITY;
+                top = fmaxf(top, s[i][x]);
+            }
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float mn = fmaxf(m[i], top);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float corr = expf(m[i] - base);
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float e = expf(s[i][x] - base);
+                sum += e;
+                ps[(ty * RPT + i) * AMS_LD + tx + 16 * x] = e;
+            }
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            l[i] = l[i] * corr + sum;
+            m[i] = mn;
+#pragma unroll
+            for (int c = 0; c < NCH; c++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[c][i][x] *= corr;
+        }
+        hidden = __syncthreads_or(hidden);  // also: K is done with, P is written
+#pragma unroll
+        for (int ch = 0; ch < NCH; ch++) {
+            if (ch) __syncthreads();
+            stage();
+            __syncthreads();
+            if (ch + 1 < NCH) fetch(V, p.ldv, ch + 1);
+            auto accumulate = [&](auto guard) {
+#pragma unroll 2
+                for (int d = 0; d < 64; d += 4) {
+                    float4 a[RPT];
+#pragma unroll
+                    for (int i = 0; i < RPT; i++) a[i] = *reinterpret_cast<const float4*>(ps + (ty * RPT + i) * AMS_LD + d);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float4 w = *reinterpret_cast<const float4*>(kv + (d + e) * AMS_LD + tx * 4);
+#pragma unroll
+                        for (int i = 0; i < RPT; i++) {
+                            const float pe = e == 0 ? a[i].x : e == 1 ? a[i].y : e == 2 ? a[i].z : a[i].w;
+                            // A hidden key's value may be anything: 0 x NaN must not reach the sum.
+                            if (!decltype(guard)::value || pe != 0.f) {
+                                o[ch][i][0] = fmaf(pe, w.x, o[ch][i][0]);
+                                o[ch][i][1] = fmaf(pe, w.y, o[ch][i][1]);
+                                o[ch][i][2] = fmaf(pe, w.z, o[ch][i][2]);
+                                o[ch][i][3] = fmaf(pe, w.w, o[ch][i][3]);
+                            }
+                        }
+                    }
+                }
+            };
+            if (hidden)
+                accumulate(std::true_type{});
+            else
+                accumulate(std::false_type{});
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+        const int rr = r0 + ty * RPT + i;
+        if (rr >= n_rows) continue;
+        const long row = sq.q0 + rr / p.G;
+        const float inv = l[i] > 0.f ? 1.f / l[i] : l[i] == 0.f ? 0.f : l[i];  // NaN stays
+        const float lse = l[i] == 0.f ? -INFINITY : m[i] + logf(l[i]);
+        if (p.nsplit > 1) {
+            const long at = ((long)split * p.q_rows + row) * p.nh + head[i];
+            if (tx == 0) p.part_lse[at] = lse;
+#pragma unroll
+            for (int c = 0; c < NCH; c++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (c * 64 + tx * 4 + x < p.hd) p.part_o[at * p.hd + c * 64 + tx * 4 + x] = o[c][i][x] * inv;
+        } else {
+            if (tx == 0 && p.lse) p.lse[row * p.nh + head[i]] = lse;
+            T* orow = (T*)p.out + row * p.ldo + (long)head[i] * p.hd;
+#pragma unroll
+            for (int c = 0; c < NCH; c++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (c * 64 + tx * 4 + x < p.hd) stf(orow, c * 64 + tx * 4 + x, o[c][i][x] * inv);
+        }
+    }
+}
+
+// Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. One warp per (row, head).
+template <typename T>
+__global__ void attention_masked_join_kernel(const MaskedParams p) {
+    const long item = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (item >= p.q_rows * p.nh) return;
+    const int lane = threadIdx.x & 31;
+    const long row = item / p.nh, step = p.q_rows * p.nh;
+    const int h = (int)(item % p.nh);
+    // Rows of no sequence were not computed: left alone.
+    int b = 0, e = p.n_seq;
+    while (b < e) {
+        const int mid = (b + e) / 2;
+        if (p.q_off[mid + 1] <= row) b = mid + 1; else e = mid;
+    }
+    if (b >= p.n_seq) return;
+    const MaskedSeq sq = masked_seq(p, b);
+    if (row < sq.q0 || row >= sq.q0 + sq.nq) return;
+    float top = -INFINITY, total = 0.f;
+    for (int s = 0; s < p.nsplit; s++) top = fmaxf(top, p.part_lse[s * step + item]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int s = 0; s < p.nsplit; s++) total += expf(p.part_lse[s * step + item] - base);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    for (int c = lane; c < p.hd; c += 32) {
+        float a = 0.f;
+        for (int s = 0; s < p.nsplit; s++) {
+            const float w = expf(p.part_lse[s * step + item] - base) * inv;
+            if (w != 0.f) a = fmaf(w, p.part_o[(s * step + item) * p.hd + c], a);
+        }
+        stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, a);
+    }
+    if (lane == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+}
+
+template <typename T, int NCH, int RPT>
+static int launch_masked_simt(const MaskedParams& p, int vec, cudaStream_t s) {
+    constexpr int TR = 16 * RPT;
+    constexpr int SMEM = (TR * (64 * NCH + 4) + 64 * AMS_LD + TR * AMS_LD + 64) * 4;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+    auto kern = attention_masked_simt_kernel<T, NCH, RPT>;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -3;
+        attr_set[dev] = true;
+    }
+    const int q_tiles = (int)(((long)p.max_q * p.G + TR - 1) / TR);
+    const long blocks = (long)q_tiles * p.n_seq * p.nkv;
+    if (blocks > 0x7fffffffL) return -1;
+    kern<<<dim3((unsigned)blocks, (unsigned)p.nsplit), 256, SMEM, s>>>(p, q_tiles, vec);
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+template <typename T>
+static int attention_masked_simt(const MaskedParams& p, int vec, cudaStream_t s) {
+    if (p.hd <= 64) return launch_masked_simt<T, 1, 4>(p, vec, s);
+    if (p.hd <= 128) return launch_masked_simt<T, 2, 4>(p, vec, s);
+    if (p.hd <= 256) return launch_masked_simt<T, 4, 4>(p, vec, s);
+    return launch_masked_simt<T, 8, 4>(p, vec, s);
+}
+
+template <typename T>
+static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
+    const long blocks = (p.q_rows * p.nh + 3) / 4;
+    if (blocks > 0x7fffffffL) return -1;
+    attention_masked_join_kernel<T><<<(unsigned)blocks, 128, 0, s>>>(p);
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// The key axis is split when the tiles alone leave most SMs idle: parts of at least 4 key tiles, at most one
+// part per idle SM.
+static int masked_splits(const eg2_masked_attention* a, int tile_rows, int tile_keys) {
+    const long G = a->nh / a->nkv;
+    const long base = ((long)a->max_q * G + tile_rows - 1) / tile_rows * a->n_seq * a->nkv;
+    const long key_tiles = ((long)a->max_k + tile_keys - 1) / tile_keys;
+    long n = num_sms() / (base > 0 ? base : 1);
+    if (n > key_tiles / 4) n = key_tiles / 4;
+    return n < 1 ? 1 : (int)n;
+}
+
+static bool masked_valid(const eg2_masked_attention* a) {
+    if (!a || (a->kind != EG2_F32 && a->kind != EG2_BF16)) return false;
+    if (a->n_seq < 0 || a->max_q < 0 || a->max_k < 0 || a->q_rows < 0 || a->k_rows < 0) return false;
+    if (a->nh <= 0 || a->nkv <= 0 || a->nh % a->nkv || a->hd <= 0 || a->hd > 512 || a->nh > 4096) return false;
+    if (a->max_q > EG2_MASKED_MAX_LEN || a->max_k > EG2_MASKED_MAX_LEN) return false;
+    if (a->ldq < (int64_t)a->nh * a->hd || a->ldo < (int64_t)a->nh * a->hd || a->ldk < (int64_t)a->nkv * a->hd ||
+        a->ldv < (int64_t)a->nkv * a->hd)
+        return false;
+    if (!std::isfinite(a->scale) || !(a->softcap >= 0.f) || !std::isfinite(a->softcap)) return false;
+    if ((a->q_doc == nullptr) != (a->k_doc == nullptr)) return false;
+    if (a->prefix_len && !a->causal) return false;
+    if (a->dist_bias && (a->dist_radius < 0 || a->dist_radius > EG2_MASKED_MAX_RADIUS)) return false;
+    if ((long)a->max_q * (a->nh / a->nkv) > 0x7fffffffL - 256) return false;
+    return true;
+}
+
+}  // namespace eg2
+
+extern "C" {
+
+int64_t eg2_attention_masked_workspace(const eg2_masked_attention* a) {
+    if (!eg2::masked_valid(a)) return EG2_ERR_INVALID;
+    const int n = eg2::masked_splits(a, 64, 64);
+    return n > 1 ? (int64_t)n * a->q_rows * a->nh * (a->hd + 1) * 4 : 0;
+}
+
+int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace eg2;
+    if (!masked_valid(a)) return EG2_ERR_INVALID;
+    if (a->q_rows == 0 || a->n_seq == 0 || a->max_q == 0) return EG2_OK;
+    if (!a->q || !a->out || !a->q_off || !a->k_off || (a->k_rows > 0 && (!a->k || !a->v))) return EG2_ERR_INVALID;
+    MaskedParams p{a->q, a->k, a->v, a->out, a->lse, a->ldq, a->ldk, a->ldv, a->ldo, a->q_off, a->k_off, a->prefix_len, a->q_doc,
+                   a->k_doc, a->slopes, a->dist_bias, a->q_rows, a->k_rows, a->n_seq, a->max_q, a->max_k, a->nh, a->nkv, a->hd,
+                   a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, a->scale, a->softcap, nullptr, nullptr};
+    cudaStream_t s = (cudaStream_t)stream;
+    p.nsplit = masked_splits(a, 64, 64);
+    if (p.nsplit > 1) {
+        if (!workspace || workspace_bytes < eg2_attention_masked_workspace(a) || (uintptr_t)workspace % 16) return EG2_ERR_INVALID;
+        p.part_o = (float*)workspace;
+        p.part_lse = p.part_o + (long)p.nsplit * p.q_rows * p.nh * p.hd;
+    }
+    const int unit = a->kind == EG2_F32 ? 16 : 8;  // bytes of four elements
+    const int vec = ((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % unit == 0 && (a->ldq | a->ldk | a->ldv | a->hd) % 4 == 0;
+    int rc = a->kind == EG2_F32 ? attention_masked_simt<float>(p, vec, s) : attention_masked_simt<bf16_t>(p, vec, s);
+    if (!rc && p.nsplit > 1) rc = a->kind == EG2_F32 ? attention_masked_join<float>(p, s) : attention_masked_join<bf16_t>(p, s);
+    if (rc == -1) return EG2_ERR_INVALID;
+    if (rc) return EG2_ERR_CUDA;
+    g_launches.fetch_add(p.nsplit > 1 ? 2 : 1, std::memory_order_relaxed);
+    return EG2_OK;
+}
+
+}  // extern "C"

@@ -11,3 +11,6 @@
 #include "noalloc.cu"
 #include "probe.cu"
 #include "runtime.cu"
+#include "rotary.cu"
+#include "attention_masked.cu"
+#include "gemm_i8.cu"

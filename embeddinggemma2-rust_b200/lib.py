@@ -31,11 +31,24 @@ _U32P = C.POINTER(C.c_uint32)
 _FP = C.POINTER(C.c_float)
 
 
+class MaskedAttention(C.Structure):
+    """``eg2_masked_attention``."""
+
+    _fields_ = [
+        ("kind", C.c_int), ("q", _P), ("k", _P), ("v", _P), ("out", _P), ("lse", _P),
+        ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("ldo", C.c_int64),
+        ("q_off", _P), ("k_off", _P), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
+        ("n_seq", C.c_int), ("max_q", C.c_int), ("max_k", C.c_int), ("nh", C.c_int), ("nkv", C.c_int), ("hd", C.c_int),
+        ("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_int), ("causal", C.c_int),
+        ("prefix_len", _P), ("q_doc", _P), ("k_doc", _P), ("slopes", _P), ("dist_bias", _P), ("dist_radius", C.c_int),
+    ]
+
+
 def exported_symbols() -> list[str]:
     """Function names declared in include/eg2.h."""
     text = HEADER.read_text()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    return re.findall(r"\b(eg2_[a-z_]+)\s*\(", text)
+    return re.findall(r"\b(eg2_[a-z0-9_]+)\s*\(", text)
 
 
 def load(build_if_missing: bool = True) -> C.CDLL:
@@ -70,6 +83,14 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         "eg2_attention_noalloc": (C.c_int, [_P, _P, _P, _P, _I32P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P]),
         "eg2_plan_passes": (C.c_int, [_I32P, C.c_int, C.c_int64, C.c_int, _I32P, _I32P]),
         "eg2_pass_policy": (C.c_int, [_P, C.POINTER(C.c_int64), C.POINTER(C.c_int)]),
+        "eg2_rotary_steps": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.POINTER(C.c_uint64), _FP]),
+        "eg2_rotary": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, C.c_int64, C.c_int, _P, C.c_int64, C.c_int, _P, C.c_int64,
+                                 _P, C.c_int64, _P, C.c_int64, C.c_int, C.c_int, _P, C.c_float, _P]),
+        "eg2_attention_masked_workspace": (C.c_int64, [C.POINTER(MaskedAttention)]),
+        "eg2_attention_masked": (C.c_int, [C.POINTER(MaskedAttention), _P, C.c_int64, _P]),
+        "eg2_quantize_rows": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int, _P]),
+        "eg2_gemm_i8": (C.c_int, [_P, C.c_int64, _P, _P, C.c_int64, _P, _P, _P, C.c_int64, C.c_int64, C.c_int, C.c_int,
+                                  C.c_int, _P]),
         "eg2_launch_count": (C.c_longlong, []),
         "eg2_device_status": (C.c_int, []),
         "eg2_device_status_reset": (None, []),

@@ -156,6 +156,80 @@ int eg2_attention(int kind, const void* q, const void* k, const void* v, void* o
 int eg2_attention_noalloc(const void* q, const void* k, const void* v, void* out, const int32_t* lens, int n_seq,
                           int nh, int nkv, int hd, int window, void* stream);
 
+/* ---- operators of one encoder layer in other forms than the two towers use ----------------------
+ * No counterpart in the reference. All three take device pointers, allocate nothing, copy nothing, run
+ * asynchronously on `stream` (NULL: the default stream) and check what the host can see before they launch
+ * (EG2_ERR_INVALID, nothing written). kind: EG2_BF16 or EG2_F32, the type of the activations; arithmetic,
+ * sums and softmax statistics are f32. Row strides are in elements; the channels of a head and the heads of
+ * a row are contiguous. */
+
+/* Rotary positions. A pair (a, b) of channels at position p becomes
+ * m (a cos t - b sin t, b cos t + a sin t), t = p f. Pair i of the rotated `rot_dim` channels is (i, i + rot_dim / 2)
+ * in the half layout, (2 i, 2 i + 1) in the interleaved one; channels from rot_dim on are passed through. */
+enum { EG2_ROTARY_HALF = 0, EG2_ROTARY_INTERLEAVED = 1 };
+/* Frequencies f_i = theta^(-2 i / rot_dim), and how they stretch by `factor` >= 1 for longer contexts: LINEAR f / factor;
+ * NTK theta * factor^(rot_dim / (rot_dim - 2)); YARN: pairs that turn more than 32 times over original_len positions
+ * stay, those that turn less than once become f / factor, a linear ramp over i between, and m = 0.1 ln(factor) + 1
+ * (m = 1 otherwise). */
+enum { EG2_SCALING_NONE = 0, EG2_SCALING_LINEAR = 1, EG2_SCALING_NTK = 2, EG2_SCALING_YARN = 3 };
+
+/* Host only: steps[rot_dim / 2] receives each pair's f in units of 2^-64 turns per position (positions times it wraps
+ * at full turns, so the angle keeps 2^-32 of a turn at any position), *magnitude the factor m. */
+int eg2_rotary_steps(int rot_dim, double theta, int scaling, double factor, double original_len, uint64_t* steps,
+                     float* magnitude);
+
+/* q [rows, nh, hd] and k [rows, nkv, hd] (either count may be 0) with row strides ldq / ldk into q_out / k_out, which may
+ * be the inputs themselves (same stride) but not overlap them otherwise. pos [rows], any int32; steps as above, on the
+ * device. inverse != 0 turns back by the same angles (the gradient of the forward form), times magnitude all the same. */
+int eg2_rotary(int kind, int layout, int inverse, const void* q, int64_t ldq, int nh, const void* k, int64_t ldk, int nkv,
+               void* q_out, int64_t ldqo, void* k_out, int64_t ldko, const int32_t* pos, int64_t rows, int hd, int rot_dim,
+               const uint64_t* steps, float magnitude, void* stream);
+
+/* Attention over packed sequences with capped, biased and masked scores.
+ *   x(i, j) = softcap tanh(scale q_i . k_j / softcap) (softcap 0: scale q_i . k_j)
+ *             - slopes[h] |j - i| + dist_bias[h][clamp(j - i, -R, R) + R]
+ *   out_i = sum_j softmax_j(x(i, j)) v_j,  lse_i = ln sum_j exp x(i, j)
+ * Sequence b has queries q_off[b] .. q_off[b + 1] and keys k_off[b] .. k_off[b + 1] (device arrays; a length may be 0);
+ * i and j are places among its keys, its queries being the last places. Query i sees key j when |j - i| <= window
+ * (window < 0: any distance), and with causal j <= i or j < prefix_len[b], and with documents q_doc[row of i] ==
+ * k_doc[row of j]. A query that sees no key gets out 0 and lse -inf; what hidden keys hold (NaN, infinities) does not
+ * reach any row. A row that sees a NaN, or an infinite value, ends NaN or infinite.
+ * hd up to 512. bf16 runs on the tensor cores when hd, the strides and the pointers are multiples of 8 elements. */
+#define EG2_MASKED_MAX_LEN (1 << 20) /* tokens of one sequence */
+#define EG2_MASKED_MAX_RADIUS 1024
+typedef struct {
+    int kind;
+    const void *q, *k, *v; /* [q_rows, nh, hd], [k_rows, nkv, hd] */
+    void* out;             /* [q_rows, nh, hd]; rows of no sequence are not written */
+    float* lse;            /* [q_rows, nh] or NULL */
+    int64_t ldq, ldk, ldv, ldo;
+    const int32_t *q_off, *k_off; /* [n_seq + 1] */
+    int64_t q_rows, k_rows;       /* rows of the buffers: no offset leads beyond them */
+    int n_seq, max_q, max_k;      /* max_q / max_k: at least the longest sequence's queries / keys */
+    int nh, nkv, hd;
+    float scale, softcap;
+    int window, causal;
+    const int32_t* prefix_len;    /* [n_seq] or NULL; causal only */
+    const int32_t *q_doc, *k_doc; /* [q_rows], [k_rows], or both NULL */
+    const float* slopes;          /* [nh] or NULL */
+    const float* dist_bias;       /* [nh, 2 dist_radius + 1] or NULL */
+    int dist_radius;
+} eg2_masked_attention;
+/* Bytes of device workspace the call needs (0 for most; calls of few queries over many keys are computed in parts that
+ * are joined through it), or a negative EG2_ERR_* code. */
+int64_t eg2_attention_masked_workspace(const eg2_masked_attention* args);
+int eg2_attention_masked(const eg2_masked_attention* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* q[r, c] = rint(x[r, c] * (127 / top)) (ties to even), scale[r] = top / 127, top = max_c |x[r, c]|. A row of zeros gets
+ * scale 0, a row with a NaN or an infinity zeros and scale NaN. Columns [k, ldq) of q are not written. */
+int eg2_quantize_rows(int kind, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int k,
+                      void* stream);
+/* C[m, n] = (sum_k A[m, k] W[n, k]) a_scale[m] w_scale[n] + bias[n] (bias may be NULL), the sum exact in 32-bit integers.
+ * C is f32 when out_f32 != 0, else bf16. Any M, N and K; A and W 16-byte aligned, lda and ldw multiples of 16. */
+#define EG2_I8_MAX_K 131072 /* 127 * 127 * K stays below 2^31 */
+int eg2_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw, const float* w_scale,
+                const float* bias, void* C, int64_t ldc, int64_t M, int N, int K, int out_f32, void* stream);
+
 /* Number of kernel launches this library has issued in the process (all contexts). */
 long long eg2_launch_count(void);
 
