@@ -10,6 +10,7 @@
 #include "common.cuh"
 #include "kernels.h"
 
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -310,6 +311,8 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
     }
 }
 
+#include "attention_masked_tc.cuh"
+
 // Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. One warp per (row, head).
 template <typename T>
 __global__ void attention_masked_join_kernel(const MaskedParams p) {
@@ -378,15 +381,30 @@ static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
     return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-// The key axis is split when the tiles alone leave most SMs idle: parts of at least 4 key tiles, at most one
-// part per idle SM.
-static int masked_splits(const eg2_masked_attention* a, int tile_rows, int tile_keys) {
-    const long G = a->nh / a->nkv;
-    const long base = ((long)a->max_q * G + tile_rows - 1) / tile_rows * a->n_seq * a->nkv;
-    const long key_tiles = ((long)a->max_k + tile_keys - 1) / tile_keys;
+// How a call runs. The tensor cores take bf16 whose rows and heads TMA can address (16-byte multiples) and G query
+// heads that divide a 128-row tile are packed into it, unless their bias tables together pass the shared memory
+// kept for them; the rest runs on the CUDA cores.
+struct MaskedPlan {
+    bool tc;
+    int Gt, nsplit;
+};
+static MaskedPlan masked_plan(const eg2_masked_attention* a) {
+    MaskedPlan r;
+    const int G = a->nh / a->nkv;
+    r.tc = a->kind == EG2_BF16 && a->hd % 8 == 0 && (a->ldq | a->ldk | a->ldv | a->ldo) % 8 == 0 &&
+           ((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) % 16 == 0 && a->k_rows > 0 &&
+           a->q_rows < (1L << 31) && a->k_rows < (1L << 31) - 128;
+    r.Gt = G;
+    if (r.tc && (128 % G || (a->dist_bias && G * (2L * a->dist_radius + 257) > AMT_TABLE))) r.Gt = 1;
+    // The key axis is split when the tiles alone leave most SMs idle: parts of at least 4 key tiles, at most one
+    // part per idle SM.
+    const int rows = !r.tc ? 64 : a->hd <= 128 ? 256 : 128, keys = r.tc ? 128 : 64;
+    const long base = ((long)a->max_q * r.Gt + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * (r.tc && a->hd > 256 ? 2 : 1);
+    const long key_tiles = ((long)a->max_k + keys - 1) / keys;
     long n = num_sms() / (base > 0 ? base : 1);
     if (n > key_tiles / 4) n = key_tiles / 4;
-    return n < 1 ? 1 : (int)n;
+    r.nsplit = n < 1 ? 1 : (int)n;
+    return r;
 }
 
 static bool masked_valid(const eg2_masked_attention* a) {
@@ -411,7 +429,7 @@ extern "C" {
 
 int64_t eg2_attention_masked_workspace(const eg2_masked_attention* a) {
     if (!eg2::masked_valid(a)) return EG2_ERR_INVALID;
-    const int n = eg2::masked_splits(a, 64, 64);
+    const int n = eg2::masked_plan(a).nsplit;
     return n > 1 ? (int64_t)n * a->q_rows * a->nh * (a->hd + 1) * 4 : 0;
 }
 
@@ -424,15 +442,22 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
                    a->k_doc, a->slopes, a->dist_bias, a->q_rows, a->k_rows, a->n_seq, a->max_q, a->max_k, a->nh, a->nkv, a->hd,
                    a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, a->scale, a->softcap, nullptr, nullptr};
     cudaStream_t s = (cudaStream_t)stream;
-    p.nsplit = masked_splits(a, 64, 64);
+    const MaskedPlan plan = masked_plan(a);
+    p.nsplit = plan.nsplit;
     if (p.nsplit > 1) {
         if (!workspace || workspace_bytes < eg2_attention_masked_workspace(a) || (uintptr_t)workspace % 16) return EG2_ERR_INVALID;
         p.part_o = (float*)workspace;
         p.part_lse = p.part_o + (long)p.nsplit * p.q_rows * p.nh * p.hd;
     }
-    const int unit = a->kind == EG2_F32 ? 16 : 8;  // bytes of four elements
-    const int vec = ((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % unit == 0 && (a->ldq | a->ldk | a->ldv | a->hd) % 4 == 0;
-    int rc = a->kind == EG2_F32 ? attention_masked_simt<float>(p, vec, s) : attention_masked_simt<bf16_t>(p, vec, s);
+    int rc;
+    if (plan.tc) {
+        rc = a->hd <= 64 ? launch_masked_tc<64>(p, plan.Gt, s) : a->hd <= 128 ? launch_masked_tc<128>(p, plan.Gt, s)
+             : a->hd <= 256 ? launch_masked_tc<256>(p, plan.Gt, s) : launch_masked_tc<512>(p, plan.Gt, s);
+    } else {
+        const int unit = a->kind == EG2_F32 ? 16 : 8;  // bytes of four elements
+        const int vec = ((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % unit == 0 && (a->ldq | a->ldk | a->ldv | a->hd) % 4 == 0;
+        rc = a->kind == EG2_F32 ? attention_masked_simt<float>(p, vec, s) : attention_masked_simt<bf16_t>(p, vec, s);
+    }
     if (!rc && p.nsplit > 1) rc = a->kind == EG2_F32 ? attention_masked_join<float>(p, s) : attention_masked_join<bf16_t>(p, s);
     if (rc == -1) return EG2_ERR_INVALID;
     if (rc) return EG2_ERR_CUDA;

@@ -1,0 +1,989 @@
+// The tensor-core form of masked attention (bf16), included by attention_masked.cu.
+//
+// A CTA holds a query tile of 128 NQ rows -- row r is token r / G, head r % G of the G query heads that share a
+// K/V head, so a K/V tile serves all of them -- and walks 128-key tiles: S = Q K^T into TMEM, the softmax warps
+// turn S into P (bf16, also in TMEM), O += P V. Persistent: one CTA per SM takes units (query tile, sequence, K/V
+// head, 256-channel half of O, part of the key axis) round robin, the heavy ones (last queries under a causal
+// mask) first.
+//
+//   HD 64, 128   NQ = 2: two 128-row tiles share every K/V tile, one softmax warpgroup each, so one tile's MMAs
+//                run under the other's softmax. TMEM: S_h [128 h, +128), O_h above; HD 64 keeps P apart from S,
+//                HD 128 has no room and writes P over the first half of its S (the next S waits for P V).
+//   HD 256, 512  NQ = 1 (O alone takes 256 columns): two S buffers [0, 128), [128, 256) by tile parity, P over S, O
+//                at [256, 512); two threads per row, 64 columns each, that swap their row maxima. HD 512 makes O
+//                256 channels at a time, each half with the whole S.
+//
+//   warp 0      TMA producer: Q, then K(0), K(1), V(0), K(2), V(1), ... into a ring of K and one of V units (one
+//               consumer each: a wait names only the parity of a barrier's phase, so whoever waits for a unit must
+//               have taken the one before it in its slot)
+//   warp 1      TMEM allocation; lane 0 issues S = Q K^T
+//   warp 2      lane 0 issues O += P V; the warp cleans V tiles (below)
+//   warp 3      scout: describes the next unit (double-buffered): the key tiles that some row may see, and those
+//               that need the document ids row by row, from the ranges of ids in the tile
+//   warps 4-11  softmax and the O / l epilogue
+//
+// The score of a pair lives in the log2 domain (scale, cap and biases carry log2 e), so a weight is one FMA and
+// one ex2. O is rescaled only when a row's maximum grows by more than 2^8: a stale maximum is exact. l sums the
+// weights in f32 as they are, P rounds them to bf16: the product with V takes 16-bit operands, and 2^-9 of a weight
+// is what the 16-bit result carries anyway.
+//
+// Hidden keys are masked by selection, so what K holds there is harmless, but a NaN or infinity in a hidden V row
+// would reach the sum as 0 x NaN. Rows past the sequence's end are zeroed in shared memory by the P V warp. Other
+// hidden rows are taken to be finite; a unit with masked tiles whose result is not finite is run once more with
+// every V tile cleaned there (non-finite elements to 0, their keys listed), and a row that sees a listed
+// key is then computed again from its visible keys alone (masked_row_again). So no visible bit depends on what
+// hidden keys hold, at no cost while all is finite.
+
+constexpr int AMT_THREADS = 384;
+constexpr int AMT_MASK_WORDS = EG2_MASKED_MAX_LEN / 128 / 32;
+constexpr int AMT_TABLE = 4096;  // floats of distance bias in shared memory
+constexpr int AMT_BAD = 64;
+constexpr float AMT_LOG2E = 1.4426950408889634f;
+
+struct alignas(16) AmtUnit {
+    MaskedSeq sq;
+    int t0, rows;     // first token of the tile; rows with a query
+    int g, head0;     // K/V head; first query head
+    int split, half;  // part of the key axis; 256-channel half of O
+    int n;            // key tiles to visit
+    int stop, scrub, retry;  // no further unit; clean every V tile; (set by the softmax) run again with scrub
+    int n_bad, pad[2];       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
+    int bad[64];
+    uint32_t visit[AMT_MASK_WORDS], docs[AMT_MASK_WORDS];
+};
+
+struct AmtParams {
+    MaskedParams p;
+    int Gt;              // query heads packed into a tile (G or 1)
+    int q_tiles, heads;  // tiles per sequence; K/V heads x (G / Gt)
+    int n_units;
+};
+
+template <int HD>
+struct AmtCfg {
+    static constexpr int NQ = HD <= 128 ? 2 : 1;
+    static constexpr int QCH = HD / 64;                   // 16 KB Q chunks per 128 rows
+    static constexpr int UCH = HD == 128 || HD == 256 ? 2 : 1;  // 64-channel chunks per ring unit (128 keys each)
+    static constexpr int UNIT = UCH * 16384;
+    static constexpr int DV = HD < 256 ? HD : 256;        // O channels per CTA
+    static constexpr int HALVES = HD / DV;
+    static constexpr int KU = HD / (64 * UCH), VU = DV / (64 * UCH);  // ring units per K / V tile
+    static constexpr int RING = HD == 64 ? 4 : 2;         // units of the K ring, and of the V ring
+    static constexpr int NC = NQ == 2 ? 128 : 64;         // S columns per softmax thread
+    static constexpr int OC = NQ == 2 ? DV : DV / 2;      // O columns per softmax thread
+    static constexpr bool OVER = HD != 64;                // P over S
+    static constexpr int T_O = HD == 64 ? 384 : 256;
+    static constexpr int O_STEP = HD == 64 ? 64 : 128;    // NQ = 2: columns between O_0 and O_1
+    static constexpr int OFF_R = NQ * QCH * 16384;
+    static constexpr int OFF_V = OFF_R + RING * UNIT;
+    static constexpr int OFF_UNIT = OFF_V + RING * UNIT;
+    static constexpr int OFF_DOC = OFF_UNIT + 2 * (int)sizeof(AmtUnit);
+    static constexpr int OFF_X = OFF_DOC + 8 * 512;
+    static constexpr int OFF_TAB = OFF_X + 2 * 2 * 128 * 4;
+    static constexpr int OFF_BAR = OFF_TAB + AMT_TABLE * 4;
+    static constexpr int N_BARS = 4 + 2 + 4 * RING + 10 + 8 + 2 + 2;
+    static constexpr int SMEM = 1024 + OFF_BAR + N_BARS * 8 + 16;
+};
+static_assert(sizeof(AmtUnit) % 16 == 0, "the staged document ids are read 16 bytes at a time");
+static_assert(AmtCfg<64>::SMEM <= 227 * 1024 && AmtCfg<128>::SMEM <= 227 * 1024 && AmtCfg<256>::SMEM <= 227 * 1024 &&
+                  AmtCfg<512>::SMEM <= 227 * 1024,
+              "masked attention: shared memory");
+
+EG2_DEV uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+EG2_DEV void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+EG2_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+EG2_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+EG2_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// tanh on |x| <= 1: x P(x^2), minimax in absolute error (2.5e-7), found by reweighted least squares.
+constexpr float AMT_T0 = 0.9999968409538269f, AMT_T1 = -0.3332400321960449f, AMT_T2 = 0.13253524899482727f,
+                AMT_T3 = -0.05097286403179169f, AMT_T4 = 0.01611418090760708f, AMT_T5 = -0.0028394656255841255f;
+EG2_DEV uint64_t tanh_small2(uint64_t x) {
+    const uint64_t y = f2_mul(x, x);
+    uint64_t r = f2_fma(y, f2_pack(AMT_T5, AMT_T5), f2_pack(AMT_T4, AMT_T4));
+    r = f2_fma(r, y, f2_pack(AMT_T3, AMT_T3));
+    r = f2_fma(r, y, f2_pack(AMT_T2, AMT_T2));
+    r = f2_fma(r, y, f2_pack(AMT_T1, AMT_T1));
+    r = f2_fma(r, y, f2_pack(AMT_T0, AMT_T0));
+    return f2_mul(x, r);
+}
+// tanh anywhere, to 2^-21 absolute: 1 - 2 / (1 + e^2x) (e^2x overflows to infinity: 1).
+EG2_DEV float tanh_any(float x) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(2.f * AMT_LOG2E * x)); }
+
+// The set bits of a mask, in order.
+struct BitWalk {
+    const uint32_t* w;
+    int at;
+    uint32_t cur;
+    EG2_DEV explicit BitWalk(const uint32_t* words) : w(words), at(0), cur(words[0]) {}
+    EG2_DEV int next() {  // there is one
+        while (!cur && at + 1 < AMT_MASK_WORDS) cur = w[++at];
+        const int b = __ffs(cur) - 1;
+        cur &= cur - 1;
+        return at * 32 + b;
+    }
+};
+
+EG2_DEV float masked_score2(const MaskedParams& p, float dot, int head, int apart) {  // in the log2 domain
+    float y = p.softcap > 0.f ? p.softcap * AMT_LOG2E * tanh_any(dot * (p.scale / p.softcap)) : dot * p.scale * AMT_LOG2E;
+    if (p.slopes) y -= p.slopes[head] * AMT_LOG2E * fabsf((float)apart);
+    if (p.table) y += p.table[(long)head * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)] * AMT_LOG2E;
+    return y;
+}
+
+// Channels [c_lo, c_hi) of one row of a unit, from its visible keys only; the whole warp works on it.
+template <int HD>
+__device__ __noinline__ void masked_row_again(const MaskedParams& p, const AmtUnit& u, int r, int Gt, int c_lo, int c_hi) {
+    constexpr int NV = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const int t = u.t0 + r / Gt, head = u.head0 + r % Gt;
+    const long row = u.sq.q0 + t;
+    const int place = u.sq.nk - u.sq.nq + t;
+    int lo, hi;
+    masked_range(p, u.sq, place, lo, hi);
+    const int qdoc = p.q_doc ? p.q_doc[row] : 0;
+    const bf16_t* q = (const bf16_t*)p.q + row * p.ldq + (long)head * p.hd;
+    float qv[NV], acc[NV], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int x = 0; x < NV; x++) {
+        qv[x] = lane + 32 * x < p.hd ? ldf(q, lane + 32 * x) : 0.f;
+        acc[x] = 0.f;
+    }
+    BitWalk walk(u.visit);
+    for (int i = 0; i < u.n; i++) {
+        const int kt = walk.next();
+        for (int key = max(lo, kt * 128); key < min(hi, kt * 128 + 128); key++) {
+            const long kr = u.sq.k0 + key;
+            if (p.k_doc && p.k_doc[kr] != qdoc) continue;
+            const bf16_t* kk = (const bf16_t*)p.k + kr * p.ldk + (long)u.g * p.hd;
+            const bf16_t* vv = (const bf16_t*)p.v + kr * p.ldv + (long)u.g * p.hd;
+            float s = 0.f;
+#pragma unroll
+            for (int x = 0; x < NV; x++)
+                if (lane + 32 * x < p.hd) s = fmaf(qv[x], ldf(kk, lane + 32 * x), s);
+            s = masked_score2(p, warp_sum(s), head, key - place);
+            const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
+            const float corr = ex2_approx(m - base), w = ex2_approx(s - base);
+            l = l * corr + w;
+            m = mn;
+#pragma unroll
+            for (int x = 0; x < NV; x++) {
+                acc[x] *= corr;
+                if (w != 0.f && lane + 32 * x < p.hd) acc[x] = fmaf(w, ldf(vv, lane + 32 * x), acc[x]);
+            }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const long at = row * p.nh + head + (p.nsplit > 1 ? (long)u.split * p.q_rows * p.nh : 0);
+#pragma unroll
+    for (int x = 0; x < NV; x++) {
+        const int c = lane + 32 * x;
+        if (c >= c_lo && c < c_hi && c < p.hd) {
+            if (p.nsplit > 1)
+                p.part_o[at * p.hd + c] = acc[x] * inv;
+            else
+                stf((bf16_t*)p.out + row * p.ldo + (long)head * p.hd, c, acc[x] * inv);
+        }
+    }
+}
+
+// Cleans one 16 KB chunk of a V tile (128 keys of 128 bytes, whatever the order of the 16-byte units in a row):
+// rows from `live` on become zero; with `scrub` non-finite elements of the others do, and their keys are listed.
+EG2_DEV void guard_chunk(uint8_t* chunk, int live, bool scrub, AmtUnit& u, int key0) {
+    const int lane = threadIdx.x & 31;
+    for (int x = lane; x < 1024; x += 32) {
+        const int row = x >> 3;
+        uint4* at = reinterpret_cast<uint4*>(chunk) + x;
+        if (row >= live) {
+            *at = make_uint4(0u, 0u, 0u, 0u);
+        } else if (scrub) {
+            uint4 v = *at;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+            bool hit = false;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                if ((w[y] & 0x7f80u) == 0x7f80u) w[y] &= 0xffff0000u, hit = true;
+                if ((w[y] & 0x7f800000u) == 0x7f800000u) w[y] &= 0xffffu, hit = true;
+            }
+            if (hit) {
+                *at = v;
+                const int n = atomicAdd(&u.n_bad, 1);  // a key may be listed more than once
+                if (n < AMT_BAD) u.bad[n] = key0 + row;
+            }
+        }
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(AMT_THREADS, 1)
+    attention_masked_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AmtParams ap) {
+    using Cfg = AmtCfg<HD>;
+    constexpr int NQ = Cfg::NQ, RING = Cfg::RING, KU = Cfg::KU, VU = Cfg::VU;
+    const MaskedParams& p = ap.p;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    AmtUnit* units = reinterpret_cast<AmtUnit*>(smem + Cfg::OFF_UNIT);
+    uint64_t* unit_full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+    uint64_t* unit_empty = unit_full + 2;
+    uint64_t* q_full = unit_empty + 2;
+    uint64_t* q_empty = q_full + 1;
+    uint64_t* k_full = q_empty + 1;
+    uint64_t* k_empty = k_full + RING;
+    uint64_t* v_full = k_empty + RING;
+    uint64_t* v_empty = v_full + RING;
+    uint64_t* s_full = v_empty + RING;
+    uint64_t* s_empty = s_full + 2;  // HD 64 only
+    uint64_t* p_full = s_empty + 2;
+    uint64_t* pv_done = p_full + 2;
+    uint64_t* o_empty = pv_done + 2;
+    uint64_t* x_bar = o_empty + 2;  // [4 lane quadrants][2 slots]: the two halves of a row meet (NQ = 1)
+    uint64_t* t_bar = x_bar + 8;    // [2]: the bias table may be rewritten; is written
+    uint64_t* drain = t_bar + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < 2; x++) {
+            mbar_init(&unit_full[x], 32);
+            mbar_init(&unit_empty[x], 11);  // TMA, both MMA issuers, 8 softmax warps
+            mbar_init(&s_full[x], 1);
+            mbar_init(&s_empty[x], 4);
+            mbar_init(&p_full[x], NQ == 2 ? 4 : 8);
+            mbar_init(&pv_done[x], 1);
+            mbar_init(&o_empty[x], NQ == 2 ? 4 : 8);
+            mbar_init(&t_bar[x], 8);
+            mbar_init(&drain[x], 1);
+        }
+        for (int x = 0; x < 8; x++) mbar_init(&x_bar[x], 2);
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int x = 0; x < RING; x++) {
+            mbar_init(&k_full[x], 1);
+            mbar_init(&k_empty[x], 1);
+            mbar_init(&v_full[x], 1);
+            mbar_init(&v_empty[x], 1);
+        }
+        *abort_flag = 0;
+        fence_mbarrier_init();
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dep_launch();
+    grid_dep_wait();
+
+    // Every role walks the scout's units; unit i's description is in units[i & 1] once unit_full says so. A role
+    // ends its walk at the last unit, or when one of its waits ran out.
+    auto unit_at = [&](int i) -> AmtUnit* {
+        if (!mbar_wait(&unit_full[i & 1], (i >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) return nullptr;
+        return units[i & 1].stop ? nullptr : &units[i & 1];
+    };
+    // Whether V of key tile kt of a unit is cleaned: rows past the sequence's end that are other sequences' (past the
+    // buffer TMA reads zeros), or a second run.
+    auto guarded = [&](const AmtUnit& u, int kt) {
+        return u.scrub || (kt * 128 + 128 > u.sq.nk && u.sq.k0 + u.sq.nk < p.k_rows);
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0 && lane == 0) {
+            int k_loads = 0, v_loads = 0, q_loads = 0;
+            bool ok = true;
+            for (int i = 0; ok; i++) {
+                const AmtUnit* un = unit_at(i);
+                if (!un) break;
+                const int n = un->n, g = un->g, half = un->half;
+                const int qrow = (int)(un->sq.q0 + un->t0), krow = (int)un->sq.k0, head0 = un->head0;
+                if (n > 0) {
+                    if (!mbar_wait(q_empty, (q_loads & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) break;
+                    mbar_arrive_expect_tx(q_full, NQ * Cfg::QCH * 16384);
+                    for (int h = 0; h < NQ; h++)
+                        for (int c = 0; c < Cfg::QCH; c++)
+                            tma_load_3d(smem + (h * Cfg::QCH + c) * 16384, &tmQ, q_full, 64 * c, head0, qrow + h * (128 / ap.Gt));
+                    q_loads++;
+                    auto load = [&](const CUtensorMap* m, uint64_t* full, uint64_t* empty, int off, int& loads, int ch, int kt) -> bool {
+                        const int u = loads % RING;
+                        if (!mbar_wait(&empty[u], ((loads / RING) & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) return false;
+                        mbar_arrive_expect_tx(&full[u], Cfg::UNIT);
+                        for (int c = 0; c < Cfg::UCH; c++)
+                            tma_load_3d(smem + off + u * Cfg::UNIT + c * 16384, m, &full[u], ch + 64 * c, g, krow + kt * 128);
+                        loads++;
+                        return true;
+                    };
+                    auto load_k = [&](int x, int kt) { return load(&tmK, k_full, k_empty, Cfg::OFF_R, k_loads, x * 64 * Cfg::UCH, kt); };
+                    auto load_v = [&](int x, int kt) { return load(&tmV, v_full, v_empty, Cfg::OFF_V, v_loads, half * 256 + x * 64 * Cfg::UCH, kt); };
+                    BitWalk walk(un->visit);
+                    int kt = walk.next();
+                    for (int x = 0; ok && x < KU; x++) ok = load_k(x, kt);
+                    for (int j = 0; ok && j < n; j++) {
+                        int kn = 0;
+                        if (j + 1 < n) {
+                            kn = walk.next();
+                            for (int x = 0; ok && x < KU; x++) ok = load_k(x, kn);
+                        }
+                        for (int x = 0; ok && x < VU; x++) ok = load_v(x, kt);
+                        kt = kn;
+                    }
+                }
+                mbar_arrive(&unit_empty[i & 1]);
+            }
+            // Every load has landed before the CTA may end (on the error path too).
+            if (q_loads) mbar_drain(q_full, (q_loads - 1) & 1, 200000000ull);
+            for (int x = max(0, k_loads - RING); x < k_loads; x++) mbar_drain(&k_full[x % RING], (x / RING) & 1, 200000000ull);
+            for (int x = max(0, v_loads - RING); x < v_loads; x++) mbar_drain(&v_full[x % RING], (x / RING) & 1, 200000000ull);
+        } else if (warp == 1 && lane == 0) {
+            constexpr uint32_t idesc = umma_idesc(128, 128, 1);
+            const uint64_t dq0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
+            const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + Cfg::OFF_R), 16, 1024);
+            int at = 0, q_seen = 0;    // at: K units taken
+            int T[2] = {0, 0};         // tiles of each half (NQ = 2), or all tiles in T[0]
+            bool ok = true;
+            for (int i = 0; ok; i++) {
+                const AmtUnit* un = unit_at(i);
+                if (!un) break;
+                const int n = un->n, nh = (NQ == 2 && un->rows > 128) ? 2 : 1;
+                if (n > 0) {
+                    ok = mbar_wait(q_full, q_seen & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    q_seen++;
+                    for (int j = 0; ok && j < n; j++) {
+                        if constexpr (NQ == 2) {
+                            if (!(ok = mbar_wait(&k_full[at % RING], (at / RING) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                            static_assert(NQ == 1 || KU == 1, "a K tile of two query tiles is one ring unit");
+                            for (int h = 0; h < nh; h++) {
+                                // S_h is free once its softmax has read it (HD 64), or P V has read the P over it.
+                                if (T[h] >= 1 && !(ok = mbar_wait(Cfg::OVER ? &pv_done[h] : &s_empty[h], (T[h] - 1) & 1,
+                                                                  EG2_DEV_TIMEOUT_ATTN, abort_flag)))
+                                    break;
+                                tc_fence_after();
+                                for (int c = 0; c < Cfg::QCH; c++)
+#pragma unroll
+                                    for (int kk = 0; kk < 4; kk++)
+                                        mma_bf16(tmem + 128 * h, dq0 + (uint64_t)((h * Cfg::QCH + c) * 1024 + 2 * kk),
+                                                 dk0 + (uint64_t)((at % RING) * (Cfg::UNIT >> 4) + c * 1024 + 2 * kk), idesc,
+                                                 (c | kk) != 0);
+                                mma_commit(&s_full[h]);
+                                T[h]++;
+                            }
+                            if (!ok) break;
+                            mma_commit(&k_empty[at % RING]);
+                            at++;
+                        } else {
+                            const int buf = T[0] & 1;
+                            if (T[0] >= 2 && !(ok = mbar_wait(&pv_done[buf], ((T[0] - 2) >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                            for (int x = 0; x < KU; x++, at++) {
+                                if (!(ok = mbar_wait(&k_full[at % RING], (at / RING) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                                tc_fence_after();
+#pragma unroll
+                                for (int c = 0; c < Cfg::UCH; c++)
+#pragma unroll
+                                    for (int kk = 0; kk < 4; kk++)
+                                        mma_bf16(tmem + 128 * buf, dq0 + (uint64_t)((x * Cfg::UCH + c) * 1024 + 2 * kk),
+                                                 dk0 + (uint64_t)((at % RING) * (Cfg::UNIT >> 4) + c * 1024 + 2 * kk), idesc,
+                                                 (x | c | kk) != 0);
+                                mma_commit(&k_empty[at % RING]);
+                            }
+                            if (!ok) break;
+                            mma_commit(&s_full[buf]);
+                            T[0]++;
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit(q_empty);
+                }
+                mbar_arrive(&unit_empty[i & 1]);
+            }
+            mma_commit(&drain[0]);
+            mbar_wait(&drain[0], 0, EG2_DEV_TIMEOUT_ATTN, nullptr);
+        } else if (warp == 2) {
+            constexpr int N = 64 * Cfg::UCH;
+            constexpr uint32_t idesc = umma_idesc(128, N, 1, /*b_mn_major=*/true);
+            const uint64_t dv0 = umma_desc_sw128(smem_u32(smem + Cfg::OFF_V), 16384, 1024);
+            int at = 0;                        // V units taken
+            int T[2] = {0, 0}, U[2] = {0, 0};  // tiles; units whose O this half has begun
+            bool ok = true;
+            for (int i = 0; ok; i++) {
+                AmtUnit* un = unit_at(i);
+                if (!un) break;
+                const int n = un->n, nh = (NQ == 2 && un->rows > 128) ? 2 : 1;
+                BitWalk walk(un->visit);
+                for (int j = 0; ok && j < n; j++) {
+                    const int kt = walk.next();
+                    const bool clean = guarded(*un, kt);
+                    for (int x = 0; ok && x < VU; x++, at++) {
+                        const int u = at % RING;
+                        if (!(ok = mbar_wait(&v_full[u], (at / RING) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                        if (clean) {
+                            for (int c = 0; c < Cfg::UCH; c++)
+                                guard_chunk(smem + Cfg::OFF_V + u * Cfg::UNIT + c * 16384, un->sq.nk - kt * 128, un->scrub, *un, kt * 128);
+                            fence_proxy_async();
+                            __syncwarp();
+                        }
+                        for (int h = 0; h < nh; h++) {
+                            const int buf = NQ == 2 ? h : T[0] & 1;
+                            if (x == 0) {
+                                const int phase = NQ == 2 ? T[h] & 1 : (T[0] >> 1) & 1;
+                                if (j == 0 && U[h] >= 1 && !(ok = mbar_wait(&o_empty[h], (U[h] - 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                                if (!(ok = mbar_wait(&p_full[buf], phase, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                            }
+                            tc_fence_after();
+                            const uint32_t tp = tmem + (Cfg::OVER ? 128 * buf : 256 + 64 * buf);
+                            if (lane == 0) {
+                                // 16 keys per MMA: 8 packed P columns, 16 V rows (2,048 bytes).
+#pragma unroll
+                                for (int kk = 0; kk < 8; kk++)
+                                    mma_bf16_ts(tmem + Cfg::T_O + h * Cfg::O_STEP + x * N, tp + 8 * kk,
+                                                dv0 + (uint64_t)(u * (Cfg::UNIT >> 4) + kk * 128), idesc, (j | kk) != 0);
+                                if (h + 1 == nh) mma_commit(&v_empty[u]);
+                                if (x + 1 == VU) mma_commit(&pv_done[buf]);
+                            }
+                            __syncwarp();
+                            if (x + 1 == VU) {
+                                T[h]++;
+                                if (j == 0) U[h]++;
+                            }
+                        }
+                    }
+                }
+                if (!ok) break;
+                if (lane == 0) mbar_arrive(&unit_empty[i & 1]);
+            }
+            if (lane == 0) {
+                mma_commit(&drain[1]);
+                mbar_wait(&drain[1], 0, EG2_DEV_TIMEOUT_ATTN, nullptr);
+            }
+        } else if (warp == 3) {
+            int id = blockIdx.x;
+            bool idle = false;
+            for (int i = 0;; i++) {
+                if (i >= 2 && !mbar_wait(&unit_empty[i & 1], ((i >> 1) & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) break;
+                AmtUnit& un = units[i & 1];
+                const bool again = i >= 2 && *(volatile int*)&un.retry;
+                __syncwarp();
+                if (again || id >= ap.n_units) {
+                    // A unit that met a value that is not finite runs again as it is described; when there is none and
+                    // none is left, an empty unit first, since the other buffer's may still have to run again.
+                    if (lane == 0) {
+                        un.stop = !again && idle;
+                        un.scrub = again;
+                        un.retry = 0;
+                        un.n_bad = 0;
+                        if (!again) un.n = un.rows = 0;
+                        if (!again && !idle) un.visit[0] = 0u;
+                    }
+                    __syncwarp();
+                    mbar_arrive(&unit_full[i & 1]);
+                    if (!again && idle) break;
+                    idle = !again;
+                    continue;
+                }
+                idle = false;
+                int x = id;
+                id += gridDim.x;
+                const int split = x % p.nsplit;
+                x /= p.nsplit;
+                const int half = x % Cfg::HALVES;
+                x /= Cfg::HALVES;
+                const int hg = x % ap.heads;
+                x /= ap.heads;
+                const int b = x % p.n_seq;
+                const int tile = ap.q_tiles - 1 - x / p.n_seq;
+                const MaskedSeq sq = masked_seq(p, b);
+                const int per = NQ * 128 / ap.Gt, t0 = tile * per;
+                const int tokens = min(per, sq.nq - t0);
+                int n = 0;
+                if (tokens > 0) {
+                    int lo, hi, tmp;
+                    masked_range(p, sq, sq.nk - sq.nq + t0, lo, tmp);
+                    masked_range(p, sq, sq.nk - sq.nq + t0 + tokens - 1, tmp, hi);
+                    const int first = lo / 128, last = hi > lo ? (hi + 127) / 128 : first;  // key tiles [first, last)
+                    int dlo = INT_MAX, dhi = INT_MIN;
+                    if (p.q_doc) {
+                        for (int t = lane; t < tokens; t += 32) {
+                            const int d = p.q_doc[sq.q0 + t0 + t];
+                            dlo = min(dlo, d);
+                            dhi = max(dhi, d);
+                        }
+                        dlo = __reduce_min_sync(0xffffffffu, dlo);
+                        dhi = __reduce_max_sync(0xffffffffu, dhi);
+                    }
+                    const int w_end = (last + 31) / 32;
+                    for (int w = lane; w <= w_end && w < AMT_MASK_WORDS; w += 32) {
+                        // bits of tiles [first, last)
+                        const int a = max(first - 32 * w, 0), z = min(last - 32 * w, 32);
+                        un.visit[w] = z > a ? (z == 32 ? 0xffffffffu : (1u << z) - 1u) & ~((1u << a) - 1u) : 0u;
+                        un.docs[w] = 0u;
+                    }
+                    __syncwarp();
+                    n = last - first;
+                    if (p.q_doc && n > 0) {
+                        n = 0;
+                        for (int w = first / 32; w < w_end; w++) {
+                            const uint32_t in = un.visit[w];
+                            uint32_t visit = 0, docs = 0;
+                            // The ids of four tiles in flight at a time.
+                            for (int t0_ = 0; t0_ < 32; t0_ += 4) {
+                                if (!((in >> t0_) & 15u)) continue;
+                                int klo[4], khi[4];
+#pragma unroll
+                                for (int t = 0; t < 4; t++) {
+                                    klo[t] = INT_MAX;
+                                    khi[t] = INT_MIN;
+#pragma unroll
+                                    for (int y = 0; y < 4; y++) {
+                                        const int key = (32 * w + t0_ + t) * 128 + 32 * y + lane;
+                                        if (key < sq.nk) {
+                                            const int d = p.k_doc[sq.k0 + key];
+                                            klo[t] = min(klo[t], d);
+                                            khi[t] = max(khi[t], d);
+                                        }
+                                    }
+                                }
+#pragma unroll
+                                for (int t = 0; t < 4; t++) {
+                                    const int a = __reduce_min_sync(0xffffffffu, klo[t]), z = __reduce_max_sync(0xffffffffu, khi[t]);
+                                    const uint32_t bit = 1u << (t0_ + t);
+                                    if (!(in & bit) || z < dlo || a > dhi) continue;
+                                    visit |= bit;
+                                    if (a != z || dlo != dhi || a != dlo) docs |= bit;
+                                }
+                            }
+                            __syncwarp();
+                            if (lane == 0) {
+                                un.visit[w] = visit;
+                                un.docs[w] = docs;
+                            }
+                            n += __popc(visit);
+                        }
+                        __syncwarp();
+                    }
+                    if (p.nsplit > 1) {
+                        // This part's share of the tiles: the a-th to the z-th of them.
+                        const int a = (int)((long)n * split / p.nsplit), z = (int)((long)n * (split + 1) / p.nsplit);
+                        int before = 0;
+                        for (int w0 = 0; w0 < w_end; w0 += 32) {
+                            const int w = w0 + lane;
+                            uint32_t v = w < w_end ? un.visit[w] : 0u;
+                            const int c = __popc(v);
+                            int sum = c;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const int y = __shfl_up_sync(0xffffffffu, sum, o);
+                                if (lane >= o) sum += y;
+                            }
+                            int at = before + sum - c;
+                            before += __shfl_sync(0xffffffffu, sum, 31);
+                            for (uint32_t left = v; left; left &= left - 1u, at++)
+                                if (at < a || at >= z) v &= ~(left & (~left + 1u));
+                            if (w < w_end) un.visit[w] = v;
+                        }
+                        n = z - a;
+                        __syncwarp();
+                    }
+                }
+                if (lane == 0) {
+                    un.sq = sq;
+                    un.t0 = t0;
+                    un.rows = max(tokens, 0) * ap.Gt;
+                    un.head0 = hg * ap.Gt;
+                    un.g = un.head0 / p.G;
+                    un.split = split;
+                    un.half = half;
+                    un.n = n;
+                    un.stop = un.scrub = un.retry = un.n_bad = 0;
+                }
+                __syncwarp();
+                mbar_arrive(&unit_full[i & 1]);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int e = warp & 3, wg = (warp - 4) >> 2;
+        const int r = 32 * e + lane;
+        const uint32_t lane_off = (uint32_t)(32 * e) << 16;
+        constexpr int NC = Cfg::NC;
+        const int col0 = NQ == 2 ? 0 : 64 * wg;  // this thread's S columns
+        int* my_docs = reinterpret_cast<int*>(smem + Cfg::OFF_DOC) + (warp - 4) * 128;
+        float* xs = reinterpret_cast<float*>(smem + Cfg::OFF_X);  // [2 slots][2 halves][128]
+        float* table = reinterpret_cast<float*>(smem + Cfg::OFF_TAB);
+        const int tab_ld = 2 * p.radius + 1 + 256;  // 128 copies of either end around the table
+        const bool capped = p.softcap > 0.f, biased = p.slopes || p.table;
+        const float in_scale = capped ? p.scale / p.softcap : p.scale * AMT_LOG2E;
+        const float cap2 = p.softcap * AMT_LOG2E;
+        // Scores are kept as v with the score v * sc: the scale is left to the exponent's FMA where nothing needs
+        // it before (sc > 0, so the order is kept).
+        const bool raw = !capped && !biased && in_scale > 0.f;
+        const float sc = raw ? in_scale : (capped && !biased) ? cap2 : 1.f;
+        int T = 0, X = 0, tab_head = -1, tables = 0;
+        bool ok = true;
+        // The two halves of a row (NQ = 1) swap a number; also the word that this half has read its part of S.
+        auto swap_halves = [&](float v) -> float {
+            xs[((X & 1) * 2 + wg) * 128 + r] = v;
+            tc_fence_before();
+            __syncwarp();
+            uint64_t* bar = &x_bar[2 * e + (X & 1)];
+            if (lane == 0) mbar_arrive(bar);
+            if (ok) ok = mbar_wait(bar, (X >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+            tc_fence_after();
+            const float other = *(volatile float*)&xs[((X & 1) * 2 + (wg ^ 1)) * 128 + r];
+            X++;
+            return other;
+        };
+
+        for (int i = 0; ok; i++) {
+            AmtUnit* un = unit_at(i);
+            if (!un) break;
+            const int n = un->n;
+            const int h = NQ == 2 ? wg : 0;
+            const int rr = 128 * h + r;
+            const bool mine = NQ == 1 || wg == 0 || un->rows > 128;  // this half takes part
+            const bool live = rr < un->rows;
+            const bool warp_live = 128 * h + 32 * e < un->rows;
+            const int tok = un->t0 + rr / ap.Gt, head = un->head0 + rr % ap.Gt;
+            const int place = un->sq.nk - un->sq.nq + tok;
+            int lo = 0, hi = 0, qdoc = 0;
+            if (live) {
+                masked_range(p, un->sq, place, lo, hi);
+                if (p.q_doc) qdoc = p.q_doc[un->sq.q0 + tok];
+            }
+            const float slope = (p.slopes && live) ? p.slopes[head] * AMT_LOG2E : 0.f;
+            if (p.table && un->rows > 0 && tab_head != un->head0) {
+                tab_head = un->head0;
+                const int s_tid = threadIdx.x - 128;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&t_bar[0]);
+                if (!(ok = mbar_wait(&t_bar[0], tables & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                for (int x = s_tid; x < ap.Gt * tab_ld; x += 256) {
+                    const int hh = x / tab_ld, c = min(max(x % tab_ld - 128, 0), 2 * p.radius);
+                    table[x] = p.table[(long)(tab_head + hh) * (2 * p.radius + 1) + c] * AMT_LOG2E;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&t_bar[1]);
+                if (!(ok = mbar_wait(&t_bar[1], tables & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                tables++;
+            }
+            const float* my_table = table + (rr % ap.Gt) * tab_ld;
+            float m = -INFINITY, l = 0.f;  // m in units of the score
+            bool any_masked = false;
+            if (mine && n > 0) {
+                BitWalk walk(un->visit);
+                for (int j = 0; j < n; j++, T++) {
+                    const int kt = walk.next();
+                    const int buf = NQ == 2 ? h : T & 1;
+                    const int phase = NQ == 2 ? T & 1 : (T >> 1) & 1;
+                    const uint32_t ts = tmem + 128 * buf + col0 + lane_off;
+                    const uint32_t tp = tmem + (Cfg::OVER ? 128 * buf + col0 / 2 : 256 + 64 * buf) + lane_off;
+                    const int kbase = kt * 128 + col0;
+                    const int lo_c = lo - kbase, hi_c = hi - kbase;  // visible columns of this thread
+                    const bool docs = p.q_doc && ((un->docs[kt >> 5] >> (kt & 31)) & 1u);
+                    const bool sees = warp_live && __any_sync(0xffffffffu, live && lo_c < NC && hi_c > 0 && lo_c < hi_c);
+                    const bool full = !docs && __all_sync(0xffffffffu, !live || (lo_c <= 0 && hi_c >= NC));
+                    any_masked |= !full;
+                    if (docs && sees) {
+#pragma unroll
+                        for (int x = 0; x < NC / 32; x++) {
+                            const int key = kbase + 32 * x + lane;
+                            my_docs[32 * x + lane] = key < un->sq.nk ? p.k_doc[un->sq.k0 + key] : 0;
+                        }
+                        __syncwarp();
+                    }
+                    if (ok) ok = mbar_wait(&s_full[buf], phase, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    tc_fence_after();
+                    float factor = 1.f, mt = -INFINITY;
+                    uint32_t su[NC];
+                    float* sv = reinterpret_cast<float*>(su);
+                    if (sees) {
+#pragma unroll
+                        for (int c = 0; c < NC / 32; c++) tmem_ld32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(su + 32 * c));
+                        tmem_ld_wait();
+                        reg_fence<NC>(su);
+                    }
+                    if constexpr (!Cfg::OVER) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&s_empty[h]);
+                    }
+                    if (sees) {
+                        if (!raw) {
+                            if (capped) {
+                                float mx = sv[0], mn = sv[0];
+#pragma unroll
+                                for (int c = 1; c < NC; c++) {
+                                    mx = fmaxf(mx, sv[c]);
+                                    mn = fminf(mn, sv[c]);
+                                }
+                                const float far = fmaxf(fabsf(mx), fabsf(mn)) * fabsf(in_scale);
+                                const uint64_t a2 = f2_pack(in_scale, in_scale);
+                                if (__all_sync(0xffffffffu, far <= 1.f)) {
+#pragma unroll
+                                    for (int c = 0; c < NC; c += 2)
+                                        f2_unpack(tanh_small2(f2_mul(f2_pack(sv[c], sv[c + 1]), a2)), sv[c], sv[c + 1]);
+                                } else {
+#pragma unroll
+                                    for (int c = 0; c < NC; c++) sv[c] = tanh_any(sv[c] * in_scale);
+                                }
+                                if (biased) {
+                                    const uint64_t c2 = f2_pack(cap2, cap2);
+#pragma unroll
+                                    for (int c = 0; c < NC; c += 2) f2_unpack(f2_mul(f2_pack(sv[c], sv[c + 1]), c2), sv[c], sv[c + 1]);
+                                }
+                            } else {
+                                const uint64_t a2 = f2_pack(in_scale, in_scale);
+#pragma unroll
+                                for (int c = 0; c < NC; c += 2) f2_unpack(f2_mul(f2_pack(sv[c], sv[c + 1]), a2), sv[c], sv[c + 1]);
+                            }
+                            if (p.slopes) {
+                                const float d0 = (float)(kbase - place);
+#pragma unroll
+                                for (int c = 0; c < NC; c++) sv[c] = fmaf(-slope, fabsf(d0 + (float)c), sv[c]);
+                            }
+                            if (p.table) {
+                                // j - i runs over NC consecutive values: clamped once, the copies of the ends do the rest.
+                                const float* tb = my_table + min(max(kbase - place, -p.radius - 128), p.radius) + p.radius + 128;
+#pragma unroll
+                                for (int c = 0; c < NC; c++) sv[c] += tb[c];
+                            }
+                        }
+                        if (!full) {
+#pragma unroll
+                            for (int c = 0; c < NC; c++) sv[c] = (c >= lo_c && c < hi_c) ? sv[c] : -INFINITY;
+                            if (docs) {
+#pragma unroll
+                                for (int c = 0; c < NC; c += 4) {
+                                    const int4 d = *reinterpret_cast<const int4*>(my_docs + c);
+                                    sv[c] = d.x == qdoc ? sv[c] : -INFINITY;
+                                    sv[c + 1] = d.y == qdoc ? sv[c + 1] : -INFINITY;
+                                    sv[c + 2] = d.z == qdoc ? sv[c + 2] : -INFINITY;
+                                    sv[c + 3] = d.w == qdoc ? sv[c + 3] : -INFINITY;
+                                }
+                                __syncwarp();
+                            }
+                        }
+                        float mx[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+                        for (int c = 4; c < NC; c++) mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+                        mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+                    }
+                    if constexpr (NQ == 1) {
+                        mt = fmaxf(mt, swap_halves(mt));
+                    }
+                    bool need = false;
+                    if (mt > m) {
+                        if (m == -INFINITY) {
+                            m = mt;
+                        } else if (mt - m > ATT_RESCALE_LOG2) {
+                            factor = ex2_approx(m - mt);
+                            m = mt;
+                            need = true;
+                        }
+                    }
+                    // O and (HD 64) P are free once the previous P V is done; with P over S and NQ = 2 a full S says so.
+                    if (j >= 1 && (!Cfg::OVER || NQ == 1)) {
+                        const int pb = NQ == 2 ? h : (T - 1) & 1, pp = NQ == 2 ? (T - 1) & 1 : ((T - 1) >> 1) & 1;
+                        if (ok) ok = mbar_wait(&pv_done[pb], pp, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                        tc_fence_after();
+                    }
+                    if (j >= 1 && __any_sync(0xffffffffu, need)) {
+                        const uint32_t to = tmem + Cfg::T_O + h * Cfg::O_STEP + (NQ == 1 ? wg * Cfg::OC : 0) + lane_off;
+#pragma unroll 1
+                        for (int c = 0; c < Cfg::OC; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + c, o);
+                            tmem_ld_wait();
+                            reg_fence<32>(o);
+#pragma unroll
+                            for (int q = 0; q < 32; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * factor);
+                            tmem_st32(to + c, o);
+                        }
+                    }
+                    l *= factor;
+                    const float base = m == -INFINITY ? 0.f : -m;
+                    if (sees) {
+                        const uint64_t sc2 = f2_pack(sc, sc), base2 = f2_pack(base, base);
+                        uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+                        for (int c = 0; c < NC; c += 32) {
+                            uint32_t pk[16];
+#pragma unroll
+                            for (int q = 0; q < 16; q++) {
+                                float a, b;
+                                f2_unpack(f2_fma(f2_pack(sv[c + 2 * q], sv[c + 2 * q + 1]), sc2, base2), a, b);
+                                a = ex2_approx(a);
+                                b = ex2_approx(b);
+                                pk[q] = bf16x2_bits(a, b);
+                                if (q & 1)
+                                    sum1 = f2_add(sum1, f2_pack(a, b));
+                                else
+                                    sum0 = f2_add(sum0, f2_pack(a, b));
+                            }
+                            tmem_st16(tp + c / 2, pk);
+                        }
+                        float a, b;
+                        f2_unpack(f2_add(sum0, sum1), a, b);
+                        l += a + b;
+                    } else if (warp_live) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int q = 0; q < 16; q++) pk[q] = 0u;
+#pragma unroll
+                        for (int c = 0; c < NC; c += 32) tmem_st16(tp + c / 2, pk);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[buf]);
+                }
+            }
+            // ---- O / l ----
+            if constexpr (NQ == 1) {
+                const float other = swap_halves(l);
+                l = wg == 0 ? l + other : other + l;  // the same sum in both
+            }
+            if (mine) {
+                if (n > 0) {
+                    const int pb = NQ == 2 ? h : (T - 1) & 1, pp = NQ == 2 ? (T - 1) & 1 : ((T - 1) >> 1) & 1;
+                    if (ok) ok = mbar_wait(&pv_done[pb], pp, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    tc_fence_after();
+                }
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const long row = un->sq.q0 + tok;
+                const long at = row * p.nh + head + (p.nsplit > 1 ? (long)un->split * p.q_rows * p.nh : 0);
+                if (live && un->half == 0 && (NQ == 2 || wg == 0)) {
+                    const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                    if (p.nsplit > 1)
+                        p.part_lse[at] = lse;
+                    else if (p.lse)
+                        p.lse[at] = lse;
+                }
+                const int ch0 = un->half * 256 + (NQ == 1 ? wg * Cfg::OC : 0);
+                const uint32_t to = tmem + Cfg::T_O + h * Cfg::O_STEP + (NQ == 1 ? wg * Cfg::OC : 0) + lane_off;
+                bool odd = false;  // some channel is not finite
+#pragma unroll 1
+                for (int c = 0; c < Cfg::OC; c += 32) {
+                    uint32_t o[32];
+                    if (n > 0 && warp_live) {
+                        tmem_ld32(to + c, o);
+                        tmem_ld_wait();
+                        reg_fence<32>(o);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 32; q++) {
+                        const float x = n > 0 && l != 0.f ? __uint_as_float(o[q]) * inv : 0.f;
+                        odd |= !(fabsf(x) < INFINITY);
+                        o[q] = __float_as_uint(x);
+                    }
+                    if (live) {
+#pragma unroll
+                        for (int q = 0; q < 32; q += 8) {
+                            const int ch = ch0 + c + q;
+                            if (ch < p.hd) {
+                                if (p.nsplit > 1) {
+                                    float4* to4 = reinterpret_cast<float4*>(p.part_o + at * p.hd + ch);
+                                    to4[0] = make_float4(__uint_as_float(o[q]), __uint_as_float(o[q + 1]), __uint_as_float(o[q + 2]),
+                                                         __uint_as_float(o[q + 3]));
+                                    to4[1] = make_float4(__uint_as_float(o[q + 4]), __uint_as_float(o[q + 5]), __uint_as_float(o[q + 6]),
+                                                         __uint_as_float(o[q + 7]));
+                                } else {
+                                    uint32_t pk[4];
+#pragma unroll
+                                    for (int y = 0; y < 4; y++)
+                                        pk[y] = bf16x2_bits(__uint_as_float(o[q + 2 * y]), __uint_as_float(o[q + 2 * y + 1]));
+                                    *reinterpret_cast<uint4*>((bf16_t*)p.out + row * p.ldo + (long)head * p.hd + ch) =
+                                        make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (n > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_empty[h]);
+                }
+                if (!un->scrub) {
+                    if (__any_sync(0xffffffffu, live && odd && any_masked) && lane == 0) *(volatile int*)&un->retry = 1;
+                } else {
+                    bool sees_bad = un->n_bad > AMT_BAD;
+                    for (int x = 0; x < min(un->n_bad, AMT_BAD); x++) {
+                        const int key = un->bad[x];
+                        sees_bad |= key >= lo && key < hi && (!p.q_doc || p.k_doc[un->sq.k0 + key] == qdoc);
+                    }
+                    uint32_t rows = __ballot_sync(0xffffffffu, live && sees_bad);
+                    while (rows) {
+                        const int b = __ffs(rows) - 1;
+                        rows &= rows - 1;
+                        masked_row_again<HD>(p, *un, 128 * h + 32 * e + b, ap.Gt, ch0, ch0 + Cfg::OC);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&unit_empty[i & 1]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int HD>
+static int launch_masked_tc(const MaskedParams& p, int Gt, cudaStream_t s) {
+    using Cfg = AmtCfg<HD>;
+    auto kern = attention_masked_tc_kernel<HD>;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM) != cudaSuccess) return -3;
+        attr_set[dev] = true;
+    }
+    CUtensorMap mq, mk, mv;
+    const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (make_tmap_3d(&mq, dt, p.q, p.hd, p.nh, p.q_rows, (uint64_t)p.hd * 2, (uint64_t)p.ldq * 2, 64, Gt, 128 / Gt) ||
+        make_tmap_3d(&mk, dt, p.k, p.hd, p.nkv, p.k_rows, (uint64_t)p.hd * 2, (uint64_t)p.ldk * 2, 64, 1, 128) ||
+        make_tmap_3d(&mv, dt, p.v, p.hd, p.nkv, p.k_rows, (uint64_t)p.hd * 2, (uint64_t)p.ldv * 2, 64, 1, 128))
+        return -1;
+    AmtParams ap;
+    ap.p = p;
+    ap.Gt = Gt;
+    ap.q_tiles = (int)(((long)p.max_q * Gt + Cfg::NQ * 128 - 1) / (Cfg::NQ * 128));
+    ap.heads = p.nh / Gt;
+    const long units = (long)ap.q_tiles * p.n_seq * ap.heads * Cfg::HALVES * p.nsplit;
+    if (units > 0x3fffffffL) return -1;
+    ap.n_units = (int)units;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)(units < num_sms() ? units : num_sms()), 1, 1);
+    cfg.blockDim = dim3(AMT_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, ap) == cudaSuccess ? 0 : -3;
+}
