@@ -398,7 +398,7 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     if (r.tc && (128 % G || (a->dist_bias && G * (2L * a->dist_radius + 257) > AMT_TABLE))) r.Gt = 1;
     // The key axis is split when the tiles alone leave most SMs idle: parts of at least 4 key tiles, at most one
     // part per idle SM.
-    const int rows = !r.tc ? 64 : a->hd <= 128 ? 256 : 128, keys = r.tc ? 128 : 64;
+    const int rows = r.tc ? 128 : 64, keys = r.tc ? 128 : 64;
     const long base = ((long)a->max_q * r.Gt + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * (r.tc && a->hd > 256 ? 2 : 1);
     const long key_tiles = ((long)a->max_k + keys - 1) / keys;
     long n = num_sms() / (base > 0 ? base : 1);

@@ -1,17 +1,15 @@
 // The tensor-core form of masked attention (bf16), included by attention_masked.cu.
 //
-// A CTA holds a query tile of 128 NQ rows -- row r is token r / G, head r % G of the G query heads that share a
-// K/V head, so a K/V tile serves all of them -- and walks 128-key tiles: S = Q K^T into TMEM, the softmax warps
-// turn S into P (bf16, also in TMEM), O += P V. Persistent: one CTA per SM takes units (query tile, sequence, K/V
-// head, 256-channel half of O, part of the key axis) round robin, the heavy ones (last queries under a causal
-// mask) first.
+// A CTA holds a query tile of 128 rows -- row r is token r / G, head r % G of the G query heads that share a K/V
+// head, so a K/V tile serves all of them -- and walks 128-key tiles: S = Q K^T into TMEM, a softmax warpgroup turns
+// S into P (bf16, written over its S), O += P V. Two softmax warpgroups take turns, one key tile each: while one
+// turns scores into weights (ex2 on the XU pipe, 8 cycles a warp) the other caps, biases and masks its tile (FMA
+// and ALU pipes). A thread holds one row; the running maximum of the row goes from one group to the other through
+// shared memory as soon as it is known. Persistent: one CTA per SM takes units (query tile, sequence, K/V head,
+// 256-channel half of O, part of the key axis), the heavy ones (last queries under a causal mask) first.
 //
-//   HD 64, 128   NQ = 2: two 128-row tiles share every K/V tile, one softmax warpgroup each, so one tile's MMAs
-//                run under the other's softmax. TMEM: S_h [128 h, +128), O_h above; HD 64 keeps P apart from S,
-//                HD 128 has no room and writes P over the first half of its S (the next S waits for P V).
-//   HD 256, 512  NQ = 1 (O alone takes 256 columns): two S buffers [0, 128), [128, 256) by tile parity, P over S, O
-//                at [256, 512); two threads per row, 64 columns each, that swap their row maxima. HD 512 makes O
-//                256 channels at a time, each half with the whole S.
+// TMEM: NS S buffers of 128 columns by tile, then O. Heads up to 128 have room for three, so S(T + 2) does not wait
+// for P(T) V; 256 and 512 for two (O takes 256 columns, at 512 channels by halves, each half with the whole S).
 //
 //   warp 0      TMA producer: Q, then K(0), K(1), V(0), K(2), V(1), ... into a ring of K and one of V units (one
 //               consumer each: a wait names only the parity of a barrier's phase, so whoever waits for a unit must
@@ -45,9 +43,9 @@ struct alignas(16) AmtUnit {
     int t0, rows;     // first token of the tile; rows with a query
     int g, head0;     // K/V head; first query head
     int split, half;  // part of the key axis; 256-channel half of O
-    int n;            // key tiles to visit
+    int n, first;     // key tiles to visit; the first (without documents they are consecutive)
     int stop, scrub, retry;  // no further unit; clean every V tile; (set by the softmax) run again with scrub
-    int n_bad, pad[2];       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
+    int n_bad, pad;       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
     int bad[64];
     uint32_t visit[AMT_MASK_WORDS], docs[AMT_MASK_WORDS];
 };
@@ -61,27 +59,25 @@ struct AmtParams {
 
 template <int HD>
 struct AmtCfg {
-    static constexpr int NQ = HD <= 128 ? 2 : 1;
-    static constexpr int QCH = HD / 64;                   // 16 KB Q chunks per 128 rows
+    static constexpr int QCH = HD / 64;                   // 16 KB chunks of Q
+    static constexpr int QBUF = HD <= 128 ? 2 : 1;        // Q buffers: the next unit's Q lands under this one
     static constexpr int UCH = HD == 128 || HD == 256 ? 2 : 1;  // 64-channel chunks per ring unit (128 keys each)
     static constexpr int UNIT = UCH * 16384;
     static constexpr int DV = HD < 256 ? HD : 256;        // O channels per CTA
     static constexpr int HALVES = HD / DV;
     static constexpr int KU = HD / (64 * UCH), VU = DV / (64 * UCH);  // ring units per K / V tile
     static constexpr int RING = HD == 64 ? 4 : 2;         // units of the K ring, and of the V ring
-    static constexpr int NC = NQ == 2 ? 128 : 64;         // S columns per softmax thread
-    static constexpr int OC = NQ == 2 ? DV : DV / 2;      // O columns per softmax thread
-    static constexpr bool OVER = HD != 64;                // P over S
-    static constexpr int T_O = HD == 64 ? 384 : 256;
-    static constexpr int O_STEP = HD == 64 ? 64 : 128;    // NQ = 2: columns between O_0 and O_1
-    static constexpr int OFF_R = NQ * QCH * 16384;
+    static constexpr int NS = HD <= 128 ? 3 : 2;          // S buffers
+    static constexpr int T_O = 128 * NS;
+    static constexpr int OC = DV / 2;                     // O columns per thread in the epilogue
+    static constexpr int OFF_R = QBUF * QCH * 16384;
     static constexpr int OFF_V = OFF_R + RING * UNIT;
     static constexpr int OFF_UNIT = OFF_V + RING * UNIT;
     static constexpr int OFF_DOC = OFF_UNIT + 2 * (int)sizeof(AmtUnit);
-    static constexpr int OFF_X = OFF_DOC + 8 * 512;
-    static constexpr int OFF_TAB = OFF_X + 2 * 2 * 128 * 4;
+    static constexpr int OFF_X = OFF_DOC + 8 * 512;       // running maxima [2][128]; (maximum, sum) [2][2 groups][128]
+    static constexpr int OFF_TAB = OFF_X + 1024 + 4096;
     static constexpr int OFF_BAR = OFF_TAB + AMT_TABLE * 4;
-    static constexpr int N_BARS = 4 + 2 + 4 * RING + 10 + 8 + 2 + 2;
+    static constexpr int N_BARS = 4 + 2 * QBUF + 4 * RING + 3 * NS + 1 + 8 + 4 + 2 + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + N_BARS * 8 + 16;
 };
 static_assert(sizeof(AmtUnit) % 16 == 0, "the staged document ids are read 16 bytes at a time");
@@ -111,20 +107,31 @@ EG2_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
     return r;
 }
 
-// tanh on |x| <= 1: x P(x^2), minimax in absolute error (2.5e-7), found by reweighted least squares.
-constexpr float AMT_T0 = 0.9999968409538269f, AMT_T1 = -0.3332400321960449f, AMT_T2 = 0.13253524899482727f,
-                AMT_T3 = -0.05097286403179169f, AMT_T4 = 0.01611418090760708f, AMT_T5 = -0.0028394656255841255f;
-EG2_DEV uint64_t tanh_small2(uint64_t x) {
-    const uint64_t y = f2_mul(x, x);
-    uint64_t r = f2_fma(y, f2_pack(AMT_T5, AMT_T5), f2_pack(AMT_T4, AMT_T4));
-    r = f2_fma(r, y, f2_pack(AMT_T3, AMT_T3));
-    r = f2_fma(r, y, f2_pack(AMT_T2, AMT_T2));
-    r = f2_fma(r, y, f2_pack(AMT_T1, AMT_T1));
-    r = f2_fma(r, y, f2_pack(AMT_T0, AMT_T0));
-    return f2_mul(x, r);
+// tanh on |x| <= 0.5: x P(x^2), minimax in relative error (3e-8 with these coefficients in f32), found by reweighted
+// least squares. Relative, because a small score's cap must not cost it digits.
+constexpr float AMT_TANH_MAX = 0.5f;
+constexpr float AMT_T0 = 1.f, AMT_T1 = -0.3333306908607483f, AMT_T2 = 0.13324779272079468f, AMT_T3 = -0.05298607423901558f,
+                AMT_T4 = 0.017135003581643105f;
+// Arrive on `bar` from one lane of a converged warp, without a branch.
+EG2_DEV void mbar_arrive_if(uint64_t* bar, bool pred) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 st;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "@p mbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"((int)pred)
+        : "memory");
 }
-// tanh anywhere, to 2^-21 absolute: 1 - 2 / (1 + e^2x) (e^2x overflows to infinity: 1).
-EG2_DEV float tanh_any(float x) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(2.f * AMT_LOG2E * x)); }
+EG2_DEV float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// tanh anywhere: past 0.5 as 1 - 2 / (1 + e^2x), good to 2^-21 there (1 where e^2x overflows).
+EG2_DEV float tanh_any(float x) {
+    const float y = x * x;
+    const float near = x * fmaf(fmaf(fmaf(fmaf(AMT_T4, y, AMT_T3), y, AMT_T2), y, AMT_T1), y, AMT_T0);
+    const float far = 1.f - __fdividef(2.f, 1.f + ex2_approx(2.f * AMT_LOG2E * x));
+    return fabsf(x) <= AMT_TANH_MAX ? near : far;
+}
 
 // The set bits of a mask, in order.
 struct BitWalk {
@@ -235,7 +242,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     attention_masked_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AmtParams ap) {
     using Cfg = AmtCfg<HD>;
-    constexpr int NQ = Cfg::NQ, RING = Cfg::RING, KU = Cfg::KU, VU = Cfg::VU;
+    constexpr int RING = Cfg::RING, KU = Cfg::KU, VU = Cfg::VU, NS = Cfg::NS, QBUF = Cfg::QBUF;
     const MaskedParams& p = ap.p;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -243,18 +250,18 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     uint64_t* unit_full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
     uint64_t* unit_empty = unit_full + 2;
     uint64_t* q_full = unit_empty + 2;
-    uint64_t* q_empty = q_full + 1;
-    uint64_t* k_full = q_empty + 1;
+    uint64_t* q_empty = q_full + QBUF;
+    uint64_t* k_full = q_empty + QBUF;
     uint64_t* k_empty = k_full + RING;
     uint64_t* v_full = k_empty + RING;
     uint64_t* v_empty = v_full + RING;
-    uint64_t* s_full = v_empty + RING;
-    uint64_t* s_empty = s_full + 2;  // HD 64 only
-    uint64_t* p_full = s_empty + 2;
-    uint64_t* pv_done = p_full + 2;
-    uint64_t* o_empty = pv_done + 2;
-    uint64_t* x_bar = o_empty + 2;  // [4 lane quadrants][2 slots]: the two halves of a row meet (NQ = 1)
-    uint64_t* t_bar = x_bar + 8;    // [2]: the bias table may be rewritten; is written
+    uint64_t* s_full = v_empty + RING;  // [NS]
+    uint64_t* p_full = s_full + NS;
+    uint64_t* pv_done = p_full + NS;
+    uint64_t* o_empty = pv_done + NS;
+    uint64_t* m_bar = o_empty + 1;  // [4 lane quadrants][2]: a row's maximum after a tile (by tile parity)
+    uint64_t* e_bar = m_bar + 8;    // [4]: the groups' maxima and sums of a unit
+    uint64_t* t_bar = e_bar + 4;    // [2]: the bias table may be rewritten; is written
     uint64_t* drain = t_bar + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -264,17 +271,21 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         for (int x = 0; x < 2; x++) {
             mbar_init(&unit_full[x], 32);
             mbar_init(&unit_empty[x], 11);  // TMA, both MMA issuers, 8 softmax warps
-            mbar_init(&s_full[x], 1);
-            mbar_init(&s_empty[x], 4);
-            mbar_init(&p_full[x], NQ == 2 ? 4 : 8);
-            mbar_init(&pv_done[x], 1);
-            mbar_init(&o_empty[x], NQ == 2 ? 4 : 8);
             mbar_init(&t_bar[x], 8);
             mbar_init(&drain[x], 1);
         }
-        for (int x = 0; x < 8; x++) mbar_init(&x_bar[x], 2);
-        mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
+        for (int x = 0; x < NS; x++) {
+            mbar_init(&s_full[x], 1);
+            mbar_init(&p_full[x], 4);
+            mbar_init(&pv_done[x], 1);
+        }
+        mbar_init(o_empty, 8);
+        for (int x = 0; x < 8; x++) mbar_init(&m_bar[x], 1);
+        for (int x = 0; x < 4; x++) mbar_init(&e_bar[x], 2);
+        for (int x = 0; x < QBUF; x++) {
+            mbar_init(&q_full[x], 1);
+            mbar_init(&q_empty[x], 1);
+        }
         for (int x = 0; x < RING; x++) {
             mbar_init(&k_full[x], 1);
             mbar_init(&k_empty[x], 1);
@@ -318,11 +329,11 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 const int n = un->n, g = un->g, half = un->half;
                 const int qrow = (int)(un->sq.q0 + un->t0), krow = (int)un->sq.k0, head0 = un->head0;
                 if (n > 0) {
-                    if (!mbar_wait(q_empty, (q_loads & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) break;
-                    mbar_arrive_expect_tx(q_full, NQ * Cfg::QCH * 16384);
-                    for (int h = 0; h < NQ; h++)
-                        for (int c = 0; c < Cfg::QCH; c++)
-                            tma_load_3d(smem + (h * Cfg::QCH + c) * 16384, &tmQ, q_full, 64 * c, head0, qrow + h * (128 / ap.Gt));
+                    const int qb = q_loads % QBUF;
+                    if (!mbar_wait(&q_empty[qb], ((q_loads / QBUF) & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) break;
+                    mbar_arrive_expect_tx(&q_full[qb], Cfg::QCH * 16384);
+                    for (int c = 0; c < Cfg::QCH; c++)
+                        tma_load_3d(smem + (qb * Cfg::QCH + c) * 16384, &tmQ, &q_full[qb], 64 * c, head0, qrow);
                     q_loads++;
                     auto load = [&](const CUtensorMap* m, uint64_t* full, uint64_t* empty, int off, int& loads, int ch, int kt) -> bool {
                         const int u = loads % RING;
@@ -351,67 +362,43 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 mbar_arrive(&unit_empty[i & 1]);
             }
             // Every load has landed before the CTA may end (on the error path too).
-            if (q_loads) mbar_drain(q_full, (q_loads - 1) & 1, 200000000ull);
+            for (int x = max(0, q_loads - QBUF); x < q_loads; x++) mbar_drain(&q_full[x % QBUF], (x / QBUF) & 1, 200000000ull);
             for (int x = max(0, k_loads - RING); x < k_loads; x++) mbar_drain(&k_full[x % RING], (x / RING) & 1, 200000000ull);
             for (int x = max(0, v_loads - RING); x < v_loads; x++) mbar_drain(&v_full[x % RING], (x / RING) & 1, 200000000ull);
         } else if (warp == 1 && lane == 0) {
             constexpr uint32_t idesc = umma_idesc(128, 128, 1);
             const uint64_t dq0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
             const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + Cfg::OFF_R), 16, 1024);
-            int at = 0, q_seen = 0;    // at: K units taken
-            int T[2] = {0, 0};         // tiles of each half (NQ = 2), or all tiles in T[0]
+            int at = 0, q_seen = 0, T = 0;  // K units, Q tiles and key tiles taken
             bool ok = true;
             for (int i = 0; ok; i++) {
                 const AmtUnit* un = unit_at(i);
                 if (!un) break;
-                const int n = un->n, nh = (NQ == 2 && un->rows > 128) ? 2 : 1;
+                const int n = un->n, qb = q_seen % QBUF;
                 if (n > 0) {
-                    ok = mbar_wait(q_full, q_seen & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    ok = mbar_wait(&q_full[qb], (q_seen / QBUF) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
                     q_seen++;
-                    for (int j = 0; ok && j < n; j++) {
-                        if constexpr (NQ == 2) {
+                    for (int j = 0; ok && j < n; j++, T++) {
+                        const int buf = T % NS;
+                        // The buffer's last P has been multiplied with V.
+                        if (T >= NS && !(ok = mbar_wait(&pv_done[buf], (T / NS - 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                        for (int x = 0; x < KU; x++, at++) {
                             if (!(ok = mbar_wait(&k_full[at % RING], (at / RING) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
-                            static_assert(NQ == 1 || KU == 1, "a K tile of two query tiles is one ring unit");
-                            for (int h = 0; h < nh; h++) {
-                                // S_h is free once its softmax has read it (HD 64), or P V has read the P over it.
-                                if (T[h] >= 1 && !(ok = mbar_wait(Cfg::OVER ? &pv_done[h] : &s_empty[h], (T[h] - 1) & 1,
-                                                                  EG2_DEV_TIMEOUT_ATTN, abort_flag)))
-                                    break;
-                                tc_fence_after();
-                                for (int c = 0; c < Cfg::QCH; c++)
+                            tc_fence_after();
 #pragma unroll
-                                    for (int kk = 0; kk < 4; kk++)
-                                        mma_bf16(tmem + 128 * h, dq0 + (uint64_t)((h * Cfg::QCH + c) * 1024 + 2 * kk),
-                                                 dk0 + (uint64_t)((at % RING) * (Cfg::UNIT >> 4) + c * 1024 + 2 * kk), idesc,
-                                                 (c | kk) != 0);
-                                mma_commit(&s_full[h]);
-                                T[h]++;
-                            }
-                            if (!ok) break;
+                            for (int c = 0; c < Cfg::UCH; c++)
+#pragma unroll
+                                for (int kk = 0; kk < 4; kk++)
+                                    mma_bf16(tmem + 128 * buf, dq0 + (uint64_t)((qb * Cfg::QCH + x * Cfg::UCH + c) * 1024 + 2 * kk),
+                                             dk0 + (uint64_t)((at % RING) * (Cfg::UNIT >> 4) + c * 1024 + 2 * kk), idesc,
+                                             (x | c | kk) != 0);
                             mma_commit(&k_empty[at % RING]);
-                            at++;
-                        } else {
-                            const int buf = T[0] & 1;
-                            if (T[0] >= 2 && !(ok = mbar_wait(&pv_done[buf], ((T[0] - 2) >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
-                            for (int x = 0; x < KU; x++, at++) {
-                                if (!(ok = mbar_wait(&k_full[at % RING], (at / RING) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
-                                tc_fence_after();
-#pragma unroll
-                                for (int c = 0; c < Cfg::UCH; c++)
-#pragma unroll
-                                    for (int kk = 0; kk < 4; kk++)
-                                        mma_bf16(tmem + 128 * buf, dq0 + (uint64_t)((x * Cfg::UCH + c) * 1024 + 2 * kk),
-                                                 dk0 + (uint64_t)((at % RING) * (Cfg::UNIT >> 4) + c * 1024 + 2 * kk), idesc,
-                                                 (x | c | kk) != 0);
-                                mma_commit(&k_empty[at % RING]);
-                            }
-                            if (!ok) break;
-                            mma_commit(&s_full[buf]);
-                            T[0]++;
                         }
+                        if (!ok) break;
+                        mma_commit(&s_full[buf]);
                     }
                     if (!ok) break;
-                    mma_commit(q_empty);
+                    mma_commit(&q_empty[qb]);
                 }
                 mbar_arrive(&unit_empty[i & 1]);
             }
@@ -421,16 +408,15 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             constexpr int N = 64 * Cfg::UCH;
             constexpr uint32_t idesc = umma_idesc(128, N, 1, /*b_mn_major=*/true);
             const uint64_t dv0 = umma_desc_sw128(smem_u32(smem + Cfg::OFF_V), 16384, 1024);
-            int at = 0;                        // V units taken
-            int T[2] = {0, 0}, U[2] = {0, 0};  // tiles; units whose O this half has begun
+            int at = 0, T = 0, U = 0;  // V units, key tiles, and units with any taken
             bool ok = true;
             for (int i = 0; ok; i++) {
                 AmtUnit* un = unit_at(i);
                 if (!un) break;
-                const int n = un->n, nh = (NQ == 2 && un->rows > 128) ? 2 : 1;
+                const int n = un->n;
                 BitWalk walk(un->visit);
-                for (int j = 0; ok && j < n; j++) {
-                    const int kt = walk.next();
+                for (int j = 0; ok && j < n; j++, T++) {
+                    const int kt = walk.next(), buf = T % NS;
                     const bool clean = guarded(*un, kt);
                     for (int x = 0; ok && x < VU; x++, at++) {
                         const int u = at % RING;
@@ -441,33 +427,26 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                             fence_proxy_async();
                             __syncwarp();
                         }
-                        for (int h = 0; h < nh; h++) {
-                            const int buf = NQ == 2 ? h : T[0] & 1;
-                            if (x == 0) {
-                                const int phase = NQ == 2 ? T[h] & 1 : (T[0] >> 1) & 1;
-                                if (j == 0 && U[h] >= 1 && !(ok = mbar_wait(&o_empty[h], (U[h] - 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
-                                if (!(ok = mbar_wait(&p_full[buf], phase, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
-                            }
-                            tc_fence_after();
-                            const uint32_t tp = tmem + (Cfg::OVER ? 128 * buf : 256 + 64 * buf);
-                            if (lane == 0) {
-                                // 16 keys per MMA: 8 packed P columns, 16 V rows (2,048 bytes).
-#pragma unroll
-                                for (int kk = 0; kk < 8; kk++)
-                                    mma_bf16_ts(tmem + Cfg::T_O + h * Cfg::O_STEP + x * N, tp + 8 * kk,
-                                                dv0 + (uint64_t)(u * (Cfg::UNIT >> 4) + kk * 128), idesc, (j | kk) != 0);
-                                if (h + 1 == nh) mma_commit(&v_empty[u]);
-                                if (x + 1 == VU) mma_commit(&pv_done[buf]);
-                            }
-                            __syncwarp();
-                            if (x + 1 == VU) {
-                                T[h]++;
-                                if (j == 0) U[h]++;
-                            }
+                        if (x == 0) {
+                            // The unit before has been read out of O.
+                            if (j == 0 && U >= 1 && !(ok = mbar_wait(o_empty, (U - 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                            if (!(ok = mbar_wait(&p_full[buf], (T / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
                         }
+                        tc_fence_after();
+                        if (lane == 0) {
+                            // 16 keys per MMA: 8 packed P columns, 16 V rows (2,048 bytes).
+#pragma unroll
+                            for (int kk = 0; kk < 8; kk++)
+                                mma_bf16_ts(tmem + Cfg::T_O + x * N, tmem + 128 * buf + 8 * kk,
+                                            dv0 + (uint64_t)(u * (Cfg::UNIT >> 4) + kk * 128), idesc, (j | kk) != 0);
+                            mma_commit(&v_empty[u]);
+                            if (x + 1 == VU) mma_commit(&pv_done[buf]);
+                        }
+                        __syncwarp();
                     }
                 }
                 if (!ok) break;
+                if (n > 0) U++;
                 if (lane == 0) mbar_arrive(&unit_empty[i & 1]);
             }
             if (lane == 0) {
@@ -477,6 +456,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         } else if (warp == 3) {
             int id = blockIdx.x;
             bool idle = false;
+            int round = 0;
             for (int i = 0;; i++) {
                 if (i >= 2 && !mbar_wait(&unit_empty[i & 1], ((i >> 1) & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) break;
                 AmtUnit& un = units[i & 1];
@@ -501,7 +481,9 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 }
                 idle = false;
                 int x = id;
-                id += gridDim.x;
+                // Round robin, every other round backwards: under a causal mask units shrink along the list.
+                round++;
+                id = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 const int split = x % p.nsplit;
                 x /= p.nsplit;
                 const int half = x % Cfg::HALVES;
@@ -511,9 +493,9 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 const int b = x % p.n_seq;
                 const int tile = ap.q_tiles - 1 - x / p.n_seq;
                 const MaskedSeq sq = masked_seq(p, b);
-                const int per = NQ * 128 / ap.Gt, t0 = tile * per;
+                const int per = 128 / ap.Gt, t0 = tile * per;
                 const int tokens = min(per, sq.nq - t0);
-                int n = 0;
+                int n = 0, first_tile = 0;
                 if (tokens > 0) {
                     int lo, hi, tmp;
                     masked_range(p, sq, sq.nk - sq.nq + t0, lo, tmp);
@@ -538,6 +520,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     }
                     __syncwarp();
                     n = last - first;
+                    first_tile = first;
                     if (p.q_doc && n > 0) {
                         n = 0;
                         for (int w = first / 32; w < w_end; w++) {
@@ -600,6 +583,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                             if (w < w_end) un.visit[w] = v;
                         }
                         n = z - a;
+                        first_tile += a;
                         __syncwarp();
                     }
                 }
@@ -612,6 +596,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     un.split = split;
                     un.half = half;
                     un.n = n;
+                    un.first = first_tile;
                     un.stop = un.scrub = un.retry = un.n_bad = 0;
                 }
                 __syncwarp();
@@ -623,45 +608,34 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const int e = warp & 3, wg = (warp - 4) >> 2;
         const int r = 32 * e + lane;
         const uint32_t lane_off = (uint32_t)(32 * e) << 16;
-        constexpr int NC = Cfg::NC;
-        const int col0 = NQ == 2 ? 0 : 64 * wg;  // this thread's S columns
+        constexpr int NC = 128;
         int* my_docs = reinterpret_cast<int*>(smem + Cfg::OFF_DOC) + (warp - 4) * 128;
-        float* xs = reinterpret_cast<float*>(smem + Cfg::OFF_X);  // [2 slots][2 halves][128]
+        float* xm = reinterpret_cast<float*>(smem + Cfg::OFF_X);  // [2][128]
+        float* xe = xm + 256;                                     // [2][2 groups][128][2]
         float* table = reinterpret_cast<float*>(smem + Cfg::OFF_TAB);
         const int tab_ld = 2 * p.radius + 1 + 256;  // 128 copies of either end around the table
-        const bool capped = p.softcap > 0.f, biased = p.slopes || p.table;
-        const float in_scale = capped ? p.scale / p.softcap : p.scale * AMT_LOG2E;
+        // Scores are kept as v with the score (log2 domain) v * sc: the scale is left to the exponent's FMA where nothing
+        // needs it before (sc > 0, so the order is kept).
+        const bool capped = p.softcap > 0.f;
         const float cap2 = p.softcap * AMT_LOG2E;
-        // Scores are kept as v with the score v * sc: the scale is left to the exponent's FMA where nothing needs
-        // it before (sc > 0, so the order is kept).
-        const bool raw = !capped && !biased && in_scale > 0.f;
-        const float sc = raw ? in_scale : (capped && !biased) ? cap2 : 1.f;
-        int T = 0, X = 0, tab_head = -1, tables = 0;
+        const float a = capped ? p.scale / p.softcap : p.scale * AMT_LOG2E;
+        const bool raw = !capped && !p.slopes && !p.table && a > 0.f;
+        const float sc = raw ? a : 1.f;
+        // cap2 tanh(a s) = s (c0 + c1 s^2 + ...) where |a s| <= 1/2, as long as the powers of a stay in range.
+        const bool near_ok = fabsf(a) > 1e-4f && fabsf(a) < 1e3f;
+        const float near_max = near_ok ? (AMT_TANH_MAX / a) * (AMT_TANH_MAX / a) : -1.f;
+        const float c0 = AMT_T0 * a * cap2, c1 = AMT_T1 * a * a * a * cap2, c2 = AMT_T2 * (a * a) * (a * a) * a * cap2,
+                    c3 = AMT_T3 * (a * a * a) * (a * a * a) * a * cap2, c4 = AMT_T4 * (a * a * a) * (a * a * a) * (a * a * a) * cap2;
+        int T = 0, U = 0, tab_head = -1, tables = 0;
         bool ok = true;
-        // The two halves of a row (NQ = 1) swap a number; also the word that this half has read its part of S.
-        auto swap_halves = [&](float v) -> float {
-            xs[((X & 1) * 2 + wg) * 128 + r] = v;
-            tc_fence_before();
-            __syncwarp();
-            uint64_t* bar = &x_bar[2 * e + (X & 1)];
-            if (lane == 0) mbar_arrive(bar);
-            if (ok) ok = mbar_wait(bar, (X >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
-            tc_fence_after();
-            const float other = *(volatile float*)&xs[((X & 1) * 2 + (wg ^ 1)) * 128 + r];
-            X++;
-            return other;
-        };
 
         for (int i = 0; ok; i++) {
             AmtUnit* un = unit_at(i);
             if (!un) break;
             const int n = un->n;
-            const int h = NQ == 2 ? wg : 0;
-            const int rr = 128 * h + r;
-            const bool mine = NQ == 1 || wg == 0 || un->rows > 128;  // this half takes part
-            const bool live = rr < un->rows;
-            const bool warp_live = 128 * h + 32 * e < un->rows;
-            const int tok = un->t0 + rr / ap.Gt, head = un->head0 + rr % ap.Gt;
+            const bool live = r < un->rows;
+            const bool warp_live = 32 * e < un->rows;
+            const int tok = un->t0 + r / ap.Gt, head = un->head0 + r % ap.Gt;
             const int place = un->sq.nk - un->sq.nq + tok;
             int lo = 0, hi = 0, qdoc = 0;
             if (live) {
@@ -684,22 +658,26 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 if (!(ok = mbar_wait(&t_bar[1], tables & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
                 tables++;
             }
-            const float* my_table = table + (rr % ap.Gt) * tab_ld;
-            float m = -INFINITY, l = 0.f;  // m in units of the score
+            const float* my_table = table + (r % ap.Gt) * tab_ld;
+            float m = -INFINITY, l = 0.f;  // this group's last maximum, and its part of the sum in units of 2^m
             bool any_masked = false;
-            if (mine && n > 0) {
+            if (n > 0) {
                 BitWalk walk(un->visit);
+                // The keys that some and that every row of the warp sees.
+                const int some_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : INT_MAX);
+                const int some_hi = __reduce_max_sync(0xffffffffu, lo < hi ? hi : 0);
+                const int all_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0);
+                const int all_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
+                const int first = un->first;
                 for (int j = 0; j < n; j++, T++) {
-                    const int kt = walk.next();
-                    const int buf = NQ == 2 ? h : T & 1;
-                    const int phase = NQ == 2 ? T & 1 : (T >> 1) & 1;
-                    const uint32_t ts = tmem + 128 * buf + col0 + lane_off;
-                    const uint32_t tp = tmem + (Cfg::OVER ? 128 * buf + col0 / 2 : 256 + 64 * buf) + lane_off;
-                    const int kbase = kt * 128 + col0;
-                    const int lo_c = lo - kbase, hi_c = hi - kbase;  // visible columns of this thread
+                    const int kt = p.q_doc ? walk.next() : first + j;
+                    if ((T & 1) != wg) continue;
+                    const int buf = T % NS;
+                    const uint32_t ts = tmem + 128 * buf + lane_off;
+                    const int kbase = kt * 128;
+                    const bool sees = kbase < some_hi && kbase + NC > some_lo;
                     const bool docs = p.q_doc && ((un->docs[kt >> 5] >> (kt & 31)) & 1u);
-                    const bool sees = warp_live && __any_sync(0xffffffffu, live && lo_c < NC && hi_c > 0 && lo_c < hi_c);
-                    const bool full = !docs && __all_sync(0xffffffffu, !live || (lo_c <= 0 && hi_c >= NC));
+                    const bool full = !docs && kbase >= all_lo && kbase + NC <= all_hi;
                     any_masked |= !full;
                     if (docs && sees) {
 #pragma unroll
@@ -709,48 +687,64 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         }
                         __syncwarp();
                     }
-                    if (ok) ok = mbar_wait(&s_full[buf], phase, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    if (ok) ok = mbar_wait(&s_full[buf], (T / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
                     tc_fence_after();
-                    float factor = 1.f, mt = -INFINITY;
+                    float mt = -INFINITY;
                     uint32_t su[NC];
                     float* sv = reinterpret_cast<float*>(su);
-                    if (sees) {
+                    auto load_s = [&] {
 #pragma unroll
                         for (int c = 0; c < NC / 32; c++) tmem_ld32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(su + 32 * c));
                         tmem_ld_wait();
                         reg_fence<NC>(su);
-                    }
-                    if constexpr (!Cfg::OVER) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&s_empty[h]);
-                    }
+                    };
                     if (sees) {
+                        load_s();
                         if (!raw) {
                             if (capped) {
-                                float mx = sv[0], mn = sv[0];
+                                // The polynomial for every score, four pairs at a time; where one is out of its range the
+                                // tile is done again from S, 16 columns at a time through TMEM.
+                                float far = 0.f;
 #pragma unroll
-                                for (int c = 1; c < NC; c++) {
-                                    mx = fmaxf(mx, sv[c]);
-                                    mn = fminf(mn, sv[c]);
+                                for (int c = 0; c < NC; c += 8) {
+                                    uint64_t x[4], y[4], r[4];
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) {
+                                        x[q] = f2_pack(sv[c + 2 * q], sv[c + 2 * q + 1]);
+                                        y[q] = f2_mul(x[q], x[q]);
+                                    }
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) {
+                                        float u, w;
+                                        f2_unpack(y[q], u, w);
+                                        far = max3(far, u, w);
+                                        r[q] = f2_fma(y[q], f2_pack(c4, c4), f2_pack(c3, c3));
+                                    }
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) r[q] = f2_fma(r[q], y[q], f2_pack(c2, c2));
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) r[q] = f2_fma(r[q], y[q], f2_pack(c1, c1));
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) r[q] = f2_fma(r[q], y[q], f2_pack(c0, c0));
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) f2_unpack(f2_mul(x[q], r[q]), sv[c + 2 * q], sv[c + 2 * q + 1]);
                                 }
-                                const float far = fmaxf(fabsf(mx), fabsf(mn)) * fabsf(in_scale);
-                                const uint64_t a2 = f2_pack(in_scale, in_scale);
-                                if (__all_sync(0xffffffffu, far <= 1.f)) {
+                                if (!__all_sync(0xffffffffu, far <= near_max)) {
+#pragma unroll 1
+                                    for (int c = 0; c < NC; c += 16) {
+                                        uint32_t o[16];
+                                        tmem_ld16(ts + c, o);
+                                        tmem_ld_wait();
+                                        reg_fence<16>(o);
 #pragma unroll
-                                    for (int c = 0; c < NC; c += 2)
-                                        f2_unpack(tanh_small2(f2_mul(f2_pack(sv[c], sv[c + 1]), a2)), sv[c], sv[c + 1]);
-                                } else {
-#pragma unroll
-                                    for (int c = 0; c < NC; c++) sv[c] = tanh_any(sv[c] * in_scale);
-                                }
-                                if (biased) {
-                                    const uint64_t c2 = f2_pack(cap2, cap2);
-#pragma unroll
-                                    for (int c = 0; c < NC; c += 2) f2_unpack(f2_mul(f2_pack(sv[c], sv[c + 1]), c2), sv[c], sv[c + 1]);
+                                        for (int q = 0; q < 16; q++) o[q] = __float_as_uint(cap2 * tanh_any(__uint_as_float(o[q]) * a));
+                                        tmem_st16(ts + c, o);
+                                    }
+                                    tmem_st_wait();
+                                    load_s();
                                 }
                             } else {
-                                const uint64_t a2 = f2_pack(in_scale, in_scale);
+                                const uint64_t a2 = f2_pack(a, a);
 #pragma unroll
                                 for (int c = 0; c < NC; c += 2) f2_unpack(f2_mul(f2_pack(sv[c], sv[c + 1]), a2), sv[c], sv[c + 1]);
                             }
@@ -760,7 +754,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                                 for (int c = 0; c < NC; c++) sv[c] = fmaf(-slope, fabsf(d0 + (float)c), sv[c]);
                             }
                             if (p.table) {
-                                // j - i runs over NC consecutive values: clamped once, the copies of the ends do the rest.
+                                // j - i runs over 128 consecutive values: clamped once, the copies of the ends do the rest.
                                 const float* tb = my_table + min(max(kbase - place, -p.radius - 128), p.radius) + p.radius + 128;
 #pragma unroll
                                 for (int c = 0; c < NC; c++) sv[c] += tb[c];
@@ -768,59 +762,66 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         }
                         if (!full) {
 #pragma unroll
-                            for (int c = 0; c < NC; c++) sv[c] = (c >= lo_c && c < hi_c) ? sv[c] : -INFINITY;
-                            if (docs) {
+                            for (int x = 0; x < NC; x += 32) {
+                                const int u = min(max(lo - kbase - x, 0), 32), z = min(max(hi - kbase - x, 0), 32);
+                                uint32_t seen = z > u ? (0xffffffffu >> (32 - z)) & (0xffffffffu << u) : 0u;
+                                if (docs) {
+                                    uint32_t same = 0;
 #pragma unroll
-                                for (int c = 0; c < NC; c += 4) {
-                                    const int4 d = *reinterpret_cast<const int4*>(my_docs + c);
-                                    sv[c] = d.x == qdoc ? sv[c] : -INFINITY;
-                                    sv[c + 1] = d.y == qdoc ? sv[c + 1] : -INFINITY;
-                                    sv[c + 2] = d.z == qdoc ? sv[c + 2] : -INFINITY;
-                                    sv[c + 3] = d.w == qdoc ? sv[c + 3] : -INFINITY;
+                                    for (int c = 0; c < 32; c += 4) {
+                                        const int4 d = *reinterpret_cast<const int4*>(my_docs + x + c);
+                                        same |= (d.x == qdoc ? 1u : 0u) << c | (d.y == qdoc ? 2u : 0u) << c | (d.z == qdoc ? 4u : 0u) << c |
+                                                (d.w == qdoc ? 8u : 0u) << c;
+                                    }
+                                    seen &= same;
                                 }
-                                __syncwarp();
+#pragma unroll
+                                for (int c = 0; c < 32; c++) sv[x + c] = (seen >> c) & 1u ? sv[x + c] : -INFINITY;
                             }
+                            if (docs) __syncwarp();
                         }
                         float mx[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
-                        for (int c = 4; c < NC; c++) mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+                        for (int c = 4; c + 7 < NC; c += 8)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) mx[q] = max3(mx[q], sv[c + q], sv[c + 4 + q]);
+#pragma unroll
+                        for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], sv[NC - 4 + q]);
                         mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
                     }
-                    if constexpr (NQ == 1) {
-                        mt = fmaxf(mt, swap_halves(mt));
+                    // The row's maximum so far comes from the other group's tile, and goes on to its next.
+                    float before = -INFINITY;
+                    if (j >= 1) {
+                        if (ok) ok = mbar_wait(&m_bar[2 * e + ((T - 1) & 1)], ((T - 1) >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                        before = *(volatile float*)&xm[((T - 1) & 1) * 128 + r];
                     }
-                    bool need = false;
-                    if (mt > m) {
-                        if (m == -INFINITY) {
-                            m = mt;
-                        } else if (mt - m > ATT_RESCALE_LOG2) {
-                            factor = ex2_approx(m - mt);
-                            m = mt;
-                            need = true;
-                        }
-                    }
-                    // O and (HD 64) P are free once the previous P V is done; with P over S and NQ = 2 a full S says so.
-                    if (j >= 1 && (!Cfg::OVER || NQ == 1)) {
-                        const int pb = NQ == 2 ? h : (T - 1) & 1, pp = NQ == 2 ? (T - 1) & 1 : ((T - 1) >> 1) & 1;
-                        if (ok) ok = mbar_wait(&pv_done[pb], pp, EG2_DEV_TIMEOUT_ATTN, abort_flag);
-                        tc_fence_after();
+                    const bool need = mt > before && before != -INFINITY && mt - before > ATT_RESCALE_LOG2;
+                    const float now = need || before == -INFINITY ? mt : before;
+                    xm[(T & 1) * 128 + r] = now;
+                    __syncwarp();
+                    mbar_arrive_if(&m_bar[2 * e + (T & 1)], lane == 0);
+                    if (now != m) {
+                        l *= ex2_approx(m - now);  // m = -inf: l is 0
+                        m = now;
                     }
                     if (j >= 1 && __any_sync(0xffffffffu, need)) {
-                        const uint32_t to = tmem + Cfg::T_O + h * Cfg::O_STEP + (NQ == 1 ? wg * Cfg::OC : 0) + lane_off;
+                        // O is in units of 2^before, and complete up to the tile before.
+                        if (ok) ok = mbar_wait(&pv_done[(T - 1) % NS], ((T - 1) / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                        tc_fence_after();
+                        const float factor = need ? ex2_approx(before - now) : 1.f;
 #pragma unroll 1
-                        for (int c = 0; c < Cfg::OC; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(to + c, o);
+                        for (int c = 0; c < Cfg::DV; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tmem + Cfg::T_O + c + lane_off, o);
                             tmem_ld_wait();
-                            reg_fence<32>(o);
+                            reg_fence<16>(o);
 #pragma unroll
-                            for (int q = 0; q < 32; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * factor);
-                            tmem_st32(to + c, o);
+                            for (int q = 0; q < 16; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * factor);
+                            tmem_st16(tmem + Cfg::T_O + c + lane_off, o);
                         }
                     }
-                    l *= factor;
-                    const float base = m == -INFINITY ? 0.f : -m;
                     if (sees) {
+                        const float base = m == -INFINITY ? 0.f : -m;
                         const uint64_t sc2 = f2_pack(sc, sc), base2 = f2_pack(base, base);
                         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
@@ -828,57 +829,69 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                             uint32_t pk[16];
 #pragma unroll
                             for (int q = 0; q < 16; q++) {
-                                float a, b;
-                                f2_unpack(f2_fma(f2_pack(sv[c + 2 * q], sv[c + 2 * q + 1]), sc2, base2), a, b);
-                                a = ex2_approx(a);
-                                b = ex2_approx(b);
-                                pk[q] = bf16x2_bits(a, b);
+                                float u, w;
+                                f2_unpack(f2_fma(f2_pack(sv[c + 2 * q], sv[c + 2 * q + 1]), sc2, base2), u, w);
+                                u = ex2_approx(u);
+                                w = ex2_approx(w);
+                                pk[q] = bf16x2_bits(u, w);
                                 if (q & 1)
-                                    sum1 = f2_add(sum1, f2_pack(a, b));
+                                    sum1 = f2_add(sum1, f2_pack(u, w));
                                 else
-                                    sum0 = f2_add(sum0, f2_pack(a, b));
+                                    sum0 = f2_add(sum0, f2_pack(u, w));
                             }
-                            tmem_st16(tp + c / 2, pk);
+                            tmem_st16(ts + c / 2, pk);
                         }
-                        float a, b;
-                        f2_unpack(f2_add(sum0, sum1), a, b);
-                        l += a + b;
+                        float u, w;
+                        f2_unpack(f2_add(sum0, sum1), u, w);
+                        l += u + w;
                     } else if (warp_live) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int q = 0; q < 16; q++) pk[q] = 0u;
 #pragma unroll
-                        for (int c = 0; c < NC; c += 32) tmem_st16(tp + c / 2, pk);
+                        for (int c = 0; c < NC; c += 32) tmem_st16(ts + c / 2, pk);
                     }
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[buf]);
+                    mbar_arrive_if(&p_full[buf], lane == 0);
                 }
             }
-            // ---- O / l ----
-            if constexpr (NQ == 1) {
-                const float other = swap_halves(l);
-                l = wg == 0 ? l + other : other + l;  // the same sum in both
+            // ---- O / l: half of the channels by each group ----
+            {
+                float* mine = xe + (((U & 1) * 2 + wg) * 128 + r) * 2;
+                float* other = xe + (((U & 1) * 2 + (wg ^ 1)) * 128 + r) * 2;
+                mine[0] = m;
+                mine[1] = l;
+                __syncwarp();
+                mbar_arrive_if(&e_bar[e], lane == 0);
+                if (ok) ok = mbar_wait(&e_bar[e], U & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                U++;
+                const float m2 = *(volatile float*)other, l2 = *(volatile float*)(other + 1);
+                const float top = fmaxf(m, m2);
+                // The same sum, in the same order, in both groups.
+                const float part = l == 0.f ? 0.f : l * (m == top ? 1.f : ex2_approx(m - top));
+                const float part2 = l2 == 0.f ? 0.f : l2 * (m2 == top ? 1.f : ex2_approx(m2 - top));
+                l = part + part2;
+                m = top;
             }
-            if (mine) {
+            {
                 if (n > 0) {
-                    const int pb = NQ == 2 ? h : (T - 1) & 1, pp = NQ == 2 ? (T - 1) & 1 : ((T - 1) >> 1) & 1;
-                    if (ok) ok = mbar_wait(&pv_done[pb], pp, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    if (ok) ok = mbar_wait(&pv_done[(T - 1) % NS], ((T - 1) / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
                     tc_fence_after();
                 }
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const long row = un->sq.q0 + tok;
                 const long at = row * p.nh + head + (p.nsplit > 1 ? (long)un->split * p.q_rows * p.nh : 0);
-                if (live && un->half == 0 && (NQ == 2 || wg == 0)) {
+                if (live && un->half == 0 && wg == 0) {
                     const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     if (p.nsplit > 1)
                         p.part_lse[at] = lse;
                     else if (p.lse)
                         p.lse[at] = lse;
                 }
-                const int ch0 = un->half * 256 + (NQ == 1 ? wg * Cfg::OC : 0);
-                const uint32_t to = tmem + Cfg::T_O + h * Cfg::O_STEP + (NQ == 1 ? wg * Cfg::OC : 0) + lane_off;
+                const int ch0 = un->half * 256 + wg * Cfg::OC;
+                const uint32_t to = tmem + Cfg::T_O + wg * Cfg::OC + lane_off;
                 bool odd = false;  // some channel is not finite
 #pragma unroll 1
                 for (int c = 0; c < Cfg::OC; c += 32) {
@@ -920,7 +933,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 if (n > 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&o_empty[h]);
+                    if (lane == 0) mbar_arrive(o_empty);
                 }
                 if (!un->scrub) {
                     if (__any_sync(0xffffffffu, live && odd && any_masked) && lane == 0) *(volatile int*)&un->retry = 1;
@@ -934,7 +947,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     while (rows) {
                         const int b = __ffs(rows) - 1;
                         rows &= rows - 1;
-                        masked_row_again<HD>(p, *un, 128 * h + 32 * e + b, ap.Gt, ch0, ch0 + Cfg::OC);
+                        masked_row_again<HD>(p, *un, 32 * e + b, ap.Gt, ch0, ch0 + Cfg::OC);
                     }
                 }
             }
@@ -970,7 +983,7 @@ static int launch_masked_tc(const MaskedParams& p, int Gt, cudaStream_t s) {
     AmtParams ap;
     ap.p = p;
     ap.Gt = Gt;
-    ap.q_tiles = (int)(((long)p.max_q * Gt + Cfg::NQ * 128 - 1) / (Cfg::NQ * 128));
+    ap.q_tiles = (int)(((long)p.max_q * Gt + 127) / 128);
     ap.heads = p.nh / Gt;
     const long units = (long)ap.q_tiles * p.n_seq * ap.heads * Cfg::HALVES * p.nsplit;
     if (units > 0x3fffffffL) return -1;
