@@ -55,6 +55,10 @@ EG2_DEV void masked_range(const MaskedParams& p, const MaskedSeq& s, int i, int&
     if (p.causal) hi = min(hi, max(i + 1, s.prefix));
 }
 
+// A distance bias as it is used: finite ones are at least -1e30, so that a row whose keys all have the type's lowest value
+// keeps its softmax (the log2 domain of the tensor-core form would overflow), -infinity hides a key.
+EG2_DEV float masked_bias(float b) { return b < -1e30f && b > -INFINITY ? -1e30f : b; }
+
 // ---------------------------------------------------------------------------------------------
 // CUDA cores, f32 arithmetic. A block takes 16 RPT rows (row r = token r / G, head r % G of the K/V head's G
 // query heads) and walks 64-key tiles; thread (ty, tx) holds RPT x 4 scores and RPT x 4 channels of each
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
                 float v = p.softcap > 0.f ? p.softcap * tanhf(s[i][x] * inv_cap) : s[i][x] * p.scale;
                 const int apart = key - place[i];
                 if (p.slopes) v -= p.slopes[head[i]] * fabsf((float)apart);
-                if (p.table) v += p.table[(long)head[i] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)];
+                if (p.table) v += masked_bias(p.table[(long)head[i] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]);
                 const bool seen = key >= lo[i] && key < hi[i] && (!p.k_doc || docs[tx + 16 * x] == qdoc[i]);
                 hidden |= !seen;
                 s[i][x] = seen ? v : -INFINITY;

@@ -37,15 +37,17 @@ constexpr int AMT_MASK_WORDS = EG2_MASKED_MAX_LEN / 128 / 32;
 constexpr int AMT_TABLE = 4096;  // floats of distance bias in shared memory
 constexpr int AMT_BAD = 64;
 constexpr float AMT_LOG2E = 1.4426950408889634f;
+constexpr float AMT_NONE = -3e38f;  // the maximum of a row that has seen nothing
 
 struct alignas(16) AmtUnit {
     MaskedSeq sq;
     int t0, rows;     // first token of the tile; rows with a query
     int g, head0;     // K/V head; first query head
     int split, half;  // part of the key axis; 256-channel half of O
-    int n, first;     // key tiles to visit; the first (without documents they are consecutive)
+    int n, first;     // key tiles to visit; the first (without documents they are consecutive,
+    int down;         // and the first `down` of them are visited backwards)
     int stop, scrub, retry;  // no further unit; clean every V tile; (set by the softmax) run again with scrub
-    int n_bad, pad;       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
+    int n_bad;       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
     int bad[64];
     uint32_t visit[AMT_MASK_WORDS], docs[AMT_MASK_WORDS];
 };
@@ -147,10 +149,22 @@ struct BitWalk {
     }
 };
 
+// A unit's key tiles in the order all roles take them.
+struct TileWalk {
+    BitWalk bits;
+    bool sparse;
+    int first, down, j;
+    EG2_DEV TileWalk(const AmtUnit& u, bool docs) : bits(u.visit), sparse(docs), first(u.first), down(u.down), j(0) {}
+    EG2_DEV int next() {
+        const int i = j++;
+        return sparse ? bits.next() : first + (i < down ? down - 1 - i : i);
+    }
+};
+
 EG2_DEV float masked_score2(const MaskedParams& p, float dot, int head, int apart) {  // in the log2 domain
     float y = p.softcap > 0.f ? p.softcap * AMT_LOG2E * tanh_any(dot * (p.scale / p.softcap)) : dot * p.scale * AMT_LOG2E;
     if (p.slopes) y -= p.slopes[head] * AMT_LOG2E * fabsf((float)apart);
-    if (p.table) y += p.table[(long)head * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)] * AMT_LOG2E;
+    if (p.table) y += masked_bias(p.table[(long)head * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]) * AMT_LOG2E;
     return y;
 }
 
@@ -172,7 +186,7 @@ __device__ __noinline__ void masked_row_again(const MaskedParams& p, const AmtUn
         qv[x] = lane + 32 * x < p.hd ? ldf(q, lane + 32 * x) : 0.f;
         acc[x] = 0.f;
     }
-    BitWalk walk(u.visit);
+    TileWalk walk(u, p.q_doc != nullptr);
     for (int i = 0; i < u.n; i++) {
         const int kt = walk.next();
         for (int key = max(lo, kt * 128); key < min(hi, kt * 128 + 128); key++) {
@@ -346,7 +360,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     };
                     auto load_k = [&](int x, int kt) { return load(&tmK, k_full, k_empty, Cfg::OFF_R, k_loads, x * 64 * Cfg::UCH, kt); };
                     auto load_v = [&](int x, int kt) { return load(&tmV, v_full, v_empty, Cfg::OFF_V, v_loads, half * 256 + x * 64 * Cfg::UCH, kt); };
-                    BitWalk walk(un->visit);
+                    TileWalk walk(*un, p.q_doc != nullptr);
                     int kt = walk.next();
                     for (int x = 0; ok && x < KU; x++) ok = load_k(x, kt);
                     for (int j = 0; ok && j < n; j++) {
@@ -414,7 +428,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 AmtUnit* un = unit_at(i);
                 if (!un) break;
                 const int n = un->n;
-                BitWalk walk(un->visit);
+                TileWalk walk(*un, p.q_doc != nullptr);
                 for (int j = 0; ok && j < n; j++, T++) {
                     const int kt = walk.next(), buf = T % NS;
                     const bool clean = guarded(*un, kt);
@@ -495,7 +509,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 const MaskedSeq sq = masked_seq(p, b);
                 const int per = 128 / ap.Gt, t0 = tile * per;
                 const int tokens = min(per, sq.nq - t0);
-                int n = 0, first_tile = 0;
+                int n = 0, first_tile = 0, down_to = -1;
                 if (tokens > 0) {
                     int lo, hi, tmp;
                     masked_range(p, sq, sq.nk - sq.nq + t0, lo, tmp);
@@ -521,6 +535,9 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     __syncwarp();
                     n = last - first;
                     first_tile = first;
+                    // Distance penalties: from the last query's place backwards, then on, so that the largest scores come
+                    // first and O is hardly ever rescaled.
+                    if (p.slopes) down_to = max(sq.nk - sq.nq + t0 + tokens - 1, 0) / 128;
                     if (p.q_doc && n > 0) {
                         n = 0;
                         for (int w = first / 32; w < w_end; w++) {
@@ -597,6 +614,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     un.half = half;
                     un.n = n;
                     un.first = first_tile;
+                    un.down = min(max(down_to + 1 - first_tile, 0), n);
                     un.stop = un.scrub = un.retry = un.n_bad = 0;
                 }
                 __syncwarp();
@@ -651,7 +669,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 if (!(ok = mbar_wait(&t_bar[0], tables & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
                 for (int x = s_tid; x < ap.Gt * tab_ld; x += 256) {
                     const int hh = x / tab_ld, c = min(max(x % tab_ld - 128, 0), 2 * p.radius);
-                    table[x] = p.table[(long)(tab_head + hh) * (2 * p.radius + 1) + c] * AMT_LOG2E;
+                    table[x] = masked_bias(p.table[(long)(tab_head + hh) * (2 * p.radius + 1) + c]) * AMT_LOG2E;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_bar[1]);
@@ -659,24 +677,24 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 tables++;
             }
             const float* my_table = table + (r % ap.Gt) * tab_ld;
-            float m = -INFINITY, l = 0.f;  // this group's last maximum, and its part of the sum in units of 2^m
+            float m = AMT_NONE, l = 0.f;  // the row's maximum at this group's last tile, and its part of the sum in units of 2^m
             bool any_masked = false;
             if (n > 0) {
-                BitWalk walk(un->visit);
+                TileWalk walk(*un, p.q_doc != nullptr);
                 // The keys that some and that every row of the warp sees.
                 const int some_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : INT_MAX);
                 const int some_hi = __reduce_max_sync(0xffffffffu, lo < hi ? hi : 0);
                 const int all_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0);
                 const int all_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
-                const int first = un->first;
-                for (int j = 0; j < n; j++, T++) {
-                    const int kt = p.q_doc ? walk.next() : first + j;
-                    if ((T & 1) != wg) continue;
-                    const int buf = T % NS;
+                const int mine = (wg ^ T) & 1;  // this group's tiles: mine, mine + 2, ...
+                if (mine) walk.next();
+                int buf = (T + mine) % NS, phase = ((T + mine) / NS) & 1;
+                for (int j = mine; j < n; j += 2) {
+                    const int tile = T + j, kbase = walk.next() * 128;
+                    if (j + 2 < n) walk.next();
                     const uint32_t ts = tmem + 128 * buf + lane_off;
-                    const int kbase = kt * 128;
                     const bool sees = kbase < some_hi && kbase + NC > some_lo;
-                    const bool docs = p.q_doc && ((un->docs[kt >> 5] >> (kt & 31)) & 1u);
+                    const bool docs = p.q_doc && ((un->docs[kbase >> 12] >> ((kbase >> 7) & 31)) & 1u);
                     const bool full = !docs && kbase >= all_lo && kbase + NC <= all_hi;
                     any_masked |= !full;
                     if (docs && sees) {
@@ -687,9 +705,9 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         }
                         __syncwarp();
                     }
-                    if (ok) ok = mbar_wait(&s_full[buf], (T / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                    if (ok) ok = mbar_wait(&s_full[buf], phase, EG2_DEV_TIMEOUT_ATTN, abort_flag);
                     tc_fence_after();
-                    float mt = -INFINITY;
+                    float mt = AMT_NONE;
                     uint32_t su[NC];
                     float* sv = reinterpret_cast<float*>(su);
                     auto load_s = [&] {
@@ -790,25 +808,22 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
                     }
                     // The row's maximum so far comes from the other group's tile, and goes on to its next.
-                    float before = -INFINITY;
+                    float before = AMT_NONE;
                     if (j >= 1) {
-                        if (ok) ok = mbar_wait(&m_bar[2 * e + ((T - 1) & 1)], ((T - 1) >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
-                        before = *(volatile float*)&xm[((T - 1) & 1) * 128 + r];
+                        if (ok) ok = mbar_wait(&m_bar[2 * e + (wg ^ 1)], ((tile - 1) >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                        before = *(volatile float*)&xm[(wg ^ 1) * 128 + r];
                     }
-                    const bool need = mt > before && before != -INFINITY && mt - before > ATT_RESCALE_LOG2;
-                    const float now = need || before == -INFINITY ? mt : before;
-                    xm[(T & 1) * 128 + r] = now;
+                    const float now = (mt - before > ATT_RESCALE_LOG2 || before == AMT_NONE) ? fmaxf(mt, AMT_NONE) : before;
+                    xm[wg * 128 + r] = now;
                     __syncwarp();
-                    mbar_arrive_if(&m_bar[2 * e + (T & 1)], lane == 0);
-                    if (now != m) {
-                        l *= ex2_approx(m - now);  // m = -inf: l is 0
-                        m = now;
-                    }
-                    if (j >= 1 && __any_sync(0xffffffffu, need)) {
+                    mbar_arrive_if(&m_bar[2 * e + wg], lane == 0);
+                    l *= ex2_approx(m - now);
+                    m = now;
+                    if (__any_sync(0xffffffffu, now != before && before != AMT_NONE)) {
                         // O is in units of 2^before, and complete up to the tile before.
-                        if (ok) ok = mbar_wait(&pv_done[(T - 1) % NS], ((T - 1) / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+                        if (ok) ok = mbar_wait(&pv_done[(tile - 1) % NS], ((tile - 1) / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
                         tc_fence_after();
-                        const float factor = need ? ex2_approx(before - now) : 1.f;
+                        const float factor = before == AMT_NONE ? 1.f : ex2_approx(before - now);
 #pragma unroll 1
                         for (int c = 0; c < Cfg::DV; c += 16) {
                             uint32_t o[16];
@@ -821,7 +836,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         }
                     }
                     if (sees) {
-                        const float base = m == -INFINITY ? 0.f : -m;
+                        const float base = -m;
                         const uint64_t sc2 = f2_pack(sc, sc), base2 = f2_pack(base, base);
                         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
@@ -855,7 +870,13 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     tc_fence_before();
                     __syncwarp();
                     mbar_arrive_if(&p_full[buf], lane == 0);
+                    buf += 2;
+                    if (buf >= NS) {
+                        buf -= NS;
+                        phase ^= 1;
+                    }
                 }
+                T += n;
             }
             // ---- O / l: half of the channels by each group ----
             {
@@ -870,9 +891,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 const float m2 = *(volatile float*)other, l2 = *(volatile float*)(other + 1);
                 const float top = fmaxf(m, m2);
                 // The same sum, in the same order, in both groups.
-                const float part = l == 0.f ? 0.f : l * (m == top ? 1.f : ex2_approx(m - top));
-                const float part2 = l2 == 0.f ? 0.f : l2 * (m2 == top ? 1.f : ex2_approx(m2 - top));
-                l = part + part2;
+                const float part = l * ex2_approx(m - top), part2 = l2 * ex2_approx(m2 - top);
+                l = wg == 0 ? part + part2 : part2 + part;
                 m = top;
             }
             {

@@ -192,7 +192,8 @@ int eg2_rotary(int kind, int layout, int inverse, const void* q, int64_t ldq, in
  * Sequence b has queries q_off[b] .. q_off[b + 1] and keys k_off[b] .. k_off[b + 1] (device arrays; a length may be 0);
  * i and j are places among its keys, its queries being the last places. Query i sees key j when |j - i| <= window
  * (window < 0: any distance), and with causal j <= i or j < prefix_len[b], and with documents q_doc[row of i] ==
- * k_doc[row of j]. A query that sees no key gets out 0 and lse -inf; what hidden keys hold (NaN, infinities) does not
+ * k_doc[row of j]. Finite entries of dist_bias below -1e30 count as -1e30 (a row that sees nothing else keeps its
+ * softmax), -infinity hides. A query that sees no key gets out 0 and lse -inf; what hidden keys hold (NaN, infinities) does not
  * reach any row. A row that sees a NaN, or an infinite value, ends NaN or infinite.
  * hd up to 512. bf16 runs on the tensor cores when hd, the strides and the pointers are multiples of 8 elements. */
 #define EG2_MASKED_MAX_LEN (1 << 20) /* tokens of one sequence */
