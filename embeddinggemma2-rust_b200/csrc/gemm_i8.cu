@@ -164,8 +164,8 @@ struct I8Cfg {
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = PAIR ? 5 : 6;
     static constexpr int OFF_OUT = STAGES * STAGE;          // per epilogue warp: two 2 KB slots
-    static constexpr int OFF_SC = OFF_OUT + 8 * 4096;       // per epilogue warp: 32 scales, 32 biases
-    static constexpr int OFF_BAR = OFF_SC + 8 * 256;
+    static constexpr int OFF_SC = OFF_OUT + 8 * 4096;       // per epilogue warp: the tile's scales and biases
+    static constexpr int OFF_BAR = OFF_SC + 8 * 8 * BN;
     static constexpr int N_BARS = 2 * STAGES + 5;
     static constexpr int SMEM = 1024 + OFF_BAR + N_BARS * 8 + 16;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
@@ -188,6 +188,15 @@ EG2_DEV void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t id
             "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
             "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
             "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
+// int to float on the integer and FMA pipes, rounded once like the conversion instruction: x = 65536 h + l with both
+// halves placed in the mantissa of 2^23. The epilogue converts every other value this way, since the conversion unit alone
+// (16 a cycle) would take as long as the MMAs of a product over K = 512.
+EG2_DEV float i32_to_f32(uint32_t x) {
+    const float l = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7410)) - 8388608.f;
+    const float h = __uint_as_float(__byte_perm(x ^ 0x80000000u, 0x4b000000u, 0x7432)) - 8421376.f;  // 2^23 + 2^15
+    return fmaf(h, 65536.f, l);
 }
 
 struct I8Params {
@@ -310,7 +319,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     } else {
         const int w = warp - 2, set = w >> 2, e = warp & 3;
         uint8_t* slots = smem + Cfg::OFF_OUT + w * 4096;
-        float* sc = reinterpret_cast<float*>(smem + Cfg::OFF_SC + w * 256);
+        float* sc = reinterpret_cast<float*>(smem + Cfg::OFF_SC + w * 8 * BN);
         int local = 0, nst = 0;
         for (int t = t_first; t < tiles; t += t_step, local++) {
             if ((local & 1) != set) continue;
@@ -318,36 +327,27 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
             const int row = row0 + lane;
             // Scales and biases of the tile's columns, requested before the sums are there.
             const float sa = row < p.M ? p.sa[row] : 0.f;
-            float sw[BN / 32], bs[BN / 32];
 #pragma unroll
-            for (int c = 0; c < BN / 32; c++) {
-                const int n = n0 + 32 * c + lane;
-                sw[c] = n < p.N ? p.sw[n] : 0.f;
-                bs[c] = (p.bias && n < p.N) ? p.bias[n] : 0.f;
+            for (int c = 0; c < BN; c += 32) {
+                const int n = n0 + c + lane;
+                sc[c + lane] = n < p.N ? p.sw[n] : 0.f;
+                sc[BN + c + lane] = (p.bias && n < p.N) ? p.bias[n] : 0.f;
             }
+            __syncwarp();
             if (!mbar_wait(&tfull[set], (local >> 1) & 1, EG2_DEV_TIMEOUT_GEMM, abort_flag)) break;
             tc_fence_after();
             const uint32_t base = tmem + set * BN + ((uint32_t)(32 * e) << 16);
-#pragma unroll
-            for (int c = 0; c < BN / 32; c++) {
-                if (n0 + 32 * c >= p.N || row0 >= p.M) break;  // the warp's rows or the columns end here
-                uint32_t r[32];
-                tmem_ld32(base + 32 * c, r);
-                sc[lane] = sw[c];
-                sc[32 + lane] = bs[c];
-                __syncwarp();
-                tmem_ld_wait();
-                reg_fence<32>(r);
+            const int chunks = row0 < p.M ? min(BN / 32, (p.N - n0 + 31) / 32) : 0;
+            auto chunk = [&](int c, uint32_t (&r)[32]) -> bool {
                 float v[32];
 #pragma unroll
                 for (int q = 0; q < 32; q += 4) {
-                    const float4 s4 = *reinterpret_cast<const float4*>(sc + q), b4 = *reinterpret_cast<const float4*>(sc + 32 + q);
+                    const float4 s4 = *reinterpret_cast<const float4*>(sc + 32 * c + q), b4 = *reinterpret_cast<const float4*>(sc + BN + 32 * c + q);
                     v[q] = fmaf((float)(int)r[q] * sa, s4.x, b4.x);
-                    v[q + 1] = fmaf((float)(int)r[q + 1] * sa, s4.y, b4.y);
+                    v[q + 1] = fmaf(i32_to_f32(r[q + 1]) * sa, s4.y, b4.y);
                     v[q + 2] = fmaf((float)(int)r[q + 2] * sa, s4.z, b4.z);
-                    v[q + 3] = fmaf((float)(int)r[q + 3] * sa, s4.w, b4.w);
+                    v[q + 3] = fmaf(i32_to_f32(r[q + 3]) * sa, s4.w, b4.w);
                 }
-                __syncwarp();
                 if (p.tma_out) {
                     if constexpr (sizeof(TO) == 2) {
                         tio_store32<2>(&tmC, slots, nst++, v, n0 + 32 * c, row0);
@@ -387,7 +387,9 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
                         __syncwarp();
                     }
                 }
-            }
+                return true;
+            };
+            if (chunks > 0) tmem_pipelined<32>(base, chunks, chunk);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {

@@ -29,15 +29,24 @@ def _bad(msg: str):
     raise L.Eg2Error(-1, msg)
 
 
-def _device(*tensors) -> int:
+try:  # the stream's handle without the Stream object around it (2 us a call)
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def _stream(first, *rest) -> int:
     """The stream to launch on, after checking that all tensors are on one CUDA device, the current one."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t.device != dev or dev.type != "cuda":
-            _bad(f"tensors must be on one CUDA device (got {[str(x.device) for x in tensors]})")
-    if dev.index != torch.cuda.current_device():
-        _bad(f"the tensors' device {dev} is not the current one")
-    return torch.cuda.current_stream(dev).cuda_stream
+    index = first.get_device()
+    for t in rest:
+        if t.get_device() != index:
+            _bad(f"tensors must be on one CUDA device (got {[str(x.device) for x in (first, *rest)]})")
+    if index < 0:
+        _bad("the tensors must be on a CUDA device")
+    if index != torch.cuda.current_device():
+        _bad(f"the tensors' device cuda:{index} is not the current one")
+    return _raw_stream(index)
 
 
 def _check(rc: int, what: str) -> None:
@@ -51,6 +60,8 @@ def _heads(t, name: str, kind=None):
         _bad(f"{name}: expected a [rows, heads, channels] tensor of {kind or 'bf16 or f32'}, got {tuple(t.shape)} {t.dtype}")
     rows, heads, hd = t.shape
     row, head, ch = t.stride()
+    if ch == 1 and head == hd and row >= heads * hd:
+        return row
     if rows and heads and hd and ((ch != 1 and hd > 1) or (head != hd and heads > 1) or (row < heads * hd and rows > 1)):
         _bad(f"{name}: the heads and channels of a row must be contiguous (strides {t.stride()})")
     return row if rows > 1 else max(row, heads * hd)
@@ -117,7 +128,7 @@ def rotary(q, k, pos, steps, *, layout: str = "half", rot_dim: int | None = None
             ldko = _heads(ko, "out k", kind)
             if ko.shape != k.shape:
                 _bad("out does not match the inputs")
-    stream = _device(q, pos, steps, qo) if k is None else _device(q, k, pos, steps, qo, ko)
+    stream = _stream(q, pos, steps, qo) if k is None else _stream(q, k, pos, steps, qo, ko)
     if rows:
         _check(L.load().eg2_rotary(KINDS[kind], LAYOUTS[layout], 1 if inverse else 0, q.data_ptr(), ldq, nh,
                                    0 if k is None else k.data_ptr(), ldk, nkv, qo.data_ptr(), ldqo,
@@ -180,7 +191,7 @@ def attention_masked(q, k, v, q_off, k_off, max_q: int, max_k: int, *, scale: fl
         if out.shape != q.shape:
             _bad("out does not match q")
         tensors.append(out)
-    stream = _device(*tensors)
+    stream = _stream(*tensors)
     lse = torch.empty((q_rows, nh), dtype=torch.float32, device=q.device) if return_lse else None
 
     def ptr(t):
@@ -216,7 +227,7 @@ def quantize_rows(x):
     ld = (k + 15) // 16 * 16
     q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    stream = _device(x)
+    stream = _stream(x)
     if rows:
         _check(L.load().eg2_quantize_rows(KINDS[x.dtype], x.data_ptr(), ldx, q.data_ptr(), ld, scale.data_ptr(), rows, k,
                                           stream), "quantize_rows")
@@ -253,9 +264,9 @@ def gemm_i8(a, a_scale, w, w_scale, *, bias=None, out_dtype=torch.bfloat16, out=
         ldc = out.stride(0) if m > 1 else max(out.stride(0), n)
     if bias is not None:
         _floats(bias, "bias", n)
-        stream = _device(a, a_scale, w, w_scale, out, bias)
+        stream = _stream(a, a_scale, w, w_scale, out, bias)
     else:
-        stream = _device(a, a_scale, w, w_scale, out)
+        stream = _stream(a, a_scale, w, w_scale, out)
     if m and n:
         _check(L.load().eg2_gemm_i8(a.data_ptr(), lda, a_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(),
                                     0 if bias is None else bias.data_ptr(), out.data_ptr(), ldc, m, n, k,
