@@ -8,138 +8,208 @@ namespace eg2 {
 // ---------------------------------------------------------------------------------------------
 // q[r, c] = rint(x[r, c] * (127 / max_c |x[r, c]|)), scale[r] = max / 127, each operation one IEEE rounding. A row
 // of zeros gets scale 0; a row that holds a NaN or an infinity gets zeros and scale NaN, so every product with it
-// is NaN. Bound by HBM: a row is read once into registers (TPR threads, NV chunks of 8 elements each), reduced and
-// written.
+// is NaN. Bound by HBM: TPR threads hold a row in registers, reduce and write it, with the next row's loads already
+// out (16,384 rows of 8,192 bf16: 402 MB). The maximum is taken over the bits of |x|, which order like the numbers and put
+// infinities and NaN above all.
 // ---------------------------------------------------------------------------------------------
+EG2_DEV uint32_t quant_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 struct QuantRow {
     float inv, scale;
+    bool bad;
 };
-EG2_DEV QuantRow quant_row(float top, bool bad) {
+EG2_DEV QuantRow quant_row(uint32_t top) {
+    const float t = __uint_as_float(top);
     QuantRow q;
-    q.inv = (bad || top == 0.f) ? 0.f : __fdiv_rn(127.f, top);
-    q.scale = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 127.f);
+    q.bad = top >= 0x7f800000u;
+    q.inv = (q.bad || top == 0u) ? 0.f : __fdiv_rn(127.f, t);
+    q.scale = q.bad ? __int_as_float(0x7fc00000) : __fdiv_rn(t, 127.f);
     return q;
 }
-EG2_DEV int quant_one(float x, const QuantRow& q, bool bad) { return bad ? 0 : __float2int_rn(__fmul_rn(x, q.inv)); }
-
-template <typename T>
-EG2_DEV void quant_load8(const T* p, int n, float (&v)[8]) {  // n of them exist; p is 16-byte aligned
-    if (n >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(p);
-            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+// rint(x * inv) in the low byte: adding 1.5 * 2^23 rounds to whole numbers, ties to even, and leaves them in the low bits of
+// the mantissa (the conversion instruction runs at an eighth of the rate).
+EG2_DEV uint32_t quant_one(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
+EG2_DEV uint32_t quant_four(const float* v, float inv) {
+    const uint32_t a = __byte_perm(quant_one(v[0], inv), quant_one(v[1], inv), 0x0040);
+    const uint32_t b = __byte_perm(quant_one(v[2], inv), quant_one(v[3], inv), 0x0040);
+    return __byte_perm(a, b, 0x5410);
+}
+// The maximum over the TPR threads of a row; slot: shared memory that the last call did not use.
+template <int TPR>
+EG2_DEV uint32_t quant_max(uint32_t top, uint32_t* slot) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = top;
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[2 * i] = __uint_as_float(u[i] << 16);
-                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        for (int i = 0; i < TPR / 32; i++) top = max(top, slot[i]);
+    }
+    return top;
+}
+
+// Eight elements as they are in memory.
+template <typename T>
+struct Quant8 {
+    uint4 u[sizeof(T) / 2];
+    EG2_DEV void load(const T* p, int n) {  // n of them exist; p is 16-byte aligned
+        if (n >= 8) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; i++) u[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+            uint32_t w[4 * sizeof(T) / 2] = {};
+            for (int i = 0; i < n; i++) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                else w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+            }
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; i++) u[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+    }
+    EG2_DEV uint32_t top() const {
+        uint32_t r = 0;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int y = 0; y < 4; y++) r = max(r, w[y] & 0x7fffffffu);
+            } else {  // two 16-bit maxima side by side
+#pragma unroll
+                for (int y = 0; y < 4; y++) r = __vmaxu2(r, w[y] & 0x7fff7fffu);
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < n ? ldf(p, i) : 0.f;
+        if constexpr (sizeof(T) == 2) r = max(r & 0xffff0000u, r << 16);
+        return r;
     }
-}
+    EG2_DEV uint2 quant(float inv) const {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                if constexpr (sizeof(T) == 4) {
+                    v[4 * i + y] = __uint_as_float(w[y]);
+                } else {
+                    v[2 * y] = __uint_as_float(w[y] << 16);
+                    v[2 * y + 1] = __uint_as_float(w[y] & 0xffff0000u);
+                }
+            }
+        }
+        return make_uint2(quant_four(v, inv), quant_four(v + 4, inv));
+    }
+};
 
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
     quantize_rows_kernel(const T* __restrict__ x, long ldx, int8_t* __restrict__ q, long ldq, float* __restrict__ scale,
                          long rows, int k) {
     grid_dep_launch();
+    grid_dep_wait();
+    __shared__ uint32_t slots[2][TPR / 32];
+    const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const long step = TPR == 32 ? (long)gridDim.x * 4 : (long)gridDim.x;
+    Quant8<T> now[NV], next[NV];
+    auto load = [&](Quant8<T> (&v)[NV], long row) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i].load(x + row * ldx + 8l * (t + i * TPR), k - 8 * (t + i * TPR));
+    };
+    long row = TPR == 32 ? (long)blockIdx.x * 4 + (threadIdx.x >> 5) : (long)blockIdx.x;
+    if (row < rows) load(now, row);
+    for (int n = 0; row < rows; row += step, n++) {
+        if (row + step < rows) load(next, row + step);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NV; i++) top = max(top, now[i].top());
+        const QuantRow qr = quant_row(quant_max<TPR>(top, slots[n & 1]));
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = 8 * (t + i * TPR);
+            if (c >= k) continue;
+            const uint2 u = qr.bad ? make_uint2(0u, 0u) : now[i].quant(qr.inv);
+            int8_t* to = q + row * ldq + c;
+            if (c + 8 <= k) {
+                *reinterpret_cast<uint2*>(to) = u;
+            } else {
+                for (int y = 0; c + y < k; y++) to[y] = (int8_t)((y < 4 ? u.x : u.y) >> (8 * (y & 3)));
+            }
+        }
+        if (t == 0) scale[row] = qr.scale;
+#pragma unroll
+        for (int i = 0; i < NV; i++) now[i] = next[i];
+    }
+}
+
+// Any alignment: TPR threads hold up to 32 single elements each.
+template <typename T, int TPR>
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
+    quantize_rows_any_kernel(const T* __restrict__ x, long ldx, int8_t* __restrict__ q, long ldq, float* __restrict__ scale,
+                             long rows, int k) {
+    grid_dep_launch();
+    grid_dep_wait();
+    __shared__ uint32_t slot[TPR / 32];
     const long row = TPR == 32 ? (long)blockIdx.x * 4 + (threadIdx.x >> 5) : (long)blockIdx.x;
     if (row >= rows) return;
     const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
     const T* xr = x + row * ldx;
-    float v[NV][8];
-    float top = 0.f;
-    bool bad = false;
+    float v[32];
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < NV; i++) quant_load8(xr + 8l * (t + i * TPR), k - 8 * (t + i * TPR), v[i]);
+    for (int i = 0; i < 32; i++) v[i] = t + i * TPR < k ? ldf(xr, t + i * TPR) : 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+    for (int i = 0; i < 32; i++) top = max(top, quant_bits(v[i]));
+    const QuantRow qr = quant_row(quant_max<TPR>(top, slot));
 #pragma unroll
-        for (int y = 0; y < 8; y++) {
-            const float a = fabsf(v[i][y]);
-            bad |= !(a < INFINITY);
-            top = fmaxf(top, a);
-        }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    bad = __any_sync(0xffffffffu, bad);
-    if constexpr (TPR > 32) {
-        __shared__ float part[TPR / 32];
-        if ((t & 31) == 0) part[t >> 5] = bad ? INFINITY : top;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < TPR / 32; i++) top = fmaxf(top, part[i]);
-        bad = top == INFINITY;
-    }
-    const QuantRow qr = quant_row(top, bad);
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = 8 * (t + i * TPR);
-        if (c >= k) continue;
-        uint32_t u[2] = {0, 0};
-#pragma unroll
-        for (int y = 0; y < 8; y++) u[y >> 2] |= (uint32_t)(quant_one(v[i][y], qr, bad) & 0xff) << (8 * (y & 3));
-        int8_t* to = q + row * ldq + c;
-        if (c + 8 <= k) {
-            *reinterpret_cast<uint2*>(to) = make_uint2(u[0], u[1]);
-        } else {
-            for (int y = 0; c + y < k; y++) to[y] = (int8_t)(u[y >> 2] >> (8 * (y & 3)));
-        }
-    }
+    for (int i = 0; i < 32; i++)
+        if (t + i * TPR < k) q[row * ldq + t + i * TPR] = qr.bad ? (int8_t)0 : (int8_t)(quant_one(v[i], qr.inv) & 0xff);
     if (t == 0) scale[row] = qr.scale;
 }
 
-// Any alignment and length: a block per row, two passes over it (the second from L1 / L2).
+// Longer rows: a block per row, two passes over it (the second from L2).
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_any_kernel(const T* __restrict__ x, long ldx, int8_t* __restrict__ q,
-                                                                long ldq, float* __restrict__ scale, int k) {
+__global__ void __launch_bounds__(512) quantize_rows_long_kernel(const T* __restrict__ x, long ldx, int8_t* __restrict__ q,
+                                                                 long ldq, float* __restrict__ scale, int k) {
     grid_dep_launch();
+    grid_dep_wait();
+    __shared__ uint32_t slot[16];
     const long row = blockIdx.x;
     const T* xr = x + row * ldx;
-    float top = 0.f;
-    for (int c = threadIdx.x; c < k; c += 256) {
-        const float a = fabsf(ldf(xr, c));
-        top = fmaxf(top, a < INFINITY ? a : INFINITY);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    __shared__ float part[8];
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = fmaxf(top, part[i]);
-    const bool bad = top == INFINITY;
-    const QuantRow qr = quant_row(top, bad);
-    for (int c = threadIdx.x; c < k; c += 256) q[row * ldq + c] = (int8_t)quant_one(ldf(xr, c), qr, bad);
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < k; c += 512) top = max(top, quant_bits(ldf(xr, c)));
+    const QuantRow qr = quant_row(quant_max<512>(top, slot));
+#pragma unroll 4
+    for (int c = threadIdx.x; c < k; c += 512) q[row * ldq + c] = qr.bad ? (int8_t)0 : (int8_t)(quant_one(ldf(xr, c), qr.inv) & 0xff);
     if (threadIdx.x == 0) scale[row] = qr.scale;
 }
 
 template <typename T>
 static int quantize_rows(const T* x, long ldx, int8_t* q, long ldq, float* scale, long rows, int k, cudaStream_t s) {
     const bool vec = (uintptr_t)x % 16 == 0 && ldx * sizeof(T) % 16 == 0 && (uintptr_t)q % 8 == 0 && ldq % 8 == 0;
-    const unsigned quarter = (unsigned)((rows + 3) / 4), each = (unsigned)rows;
-    if (!vec || k > 16384)
-        quantize_rows_any_kernel<T><<<each, 256, 0, s>>>(x, ldx, q, ldq, scale, k);
-    else if (k <= 256)
-        quantize_rows_kernel<T, 32, 1><<<quarter, 128, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    else if (k <= 512)
-        quantize_rows_kernel<T, 32, 2><<<quarter, 128, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    else if (k <= 1024)
-        quantize_rows_kernel<T, 32, 4><<<quarter, 128, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    else if (k <= 2048)
-        quantize_rows_kernel<T, 128, 2><<<each, 128, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    else if (k <= 4096)
-        quantize_rows_kernel<T, 256, 2><<<each, 256, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    else if (k <= 8192)
-        quantize_rows_kernel<T, 256, 4><<<each, 256, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    else
-        quantize_rows_kernel<T, 512, 4><<<each, 512, 0, s>>>(x, ldx, q, ldq, scale, rows, k);
-    return cudaGetLastError() == cudaSuccess ? 0 : -3;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    auto run = [&](auto kern, int tpr, bool walk, auto... args) {
+        // Walking kernels: as many threads as are resident, 1,024 to 2,048 an SM by their registers.
+        const long units = tpr == 32 ? (rows + 3) / 4 : rows, most = (long)num_sms() * 2048 / (tpr == 32 ? 128 : tpr);
+        cfg.gridDim = dim3((unsigned)(walk && units > most ? most : units), 1, 1);
+        cfg.blockDim = dim3(tpr == 32 ? 128 : tpr, 1, 1);
+        return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? 0 : -3;
+    };
+    if (vec && k <= 256) return run(quantize_rows_kernel<T, 32, 1>, 32, true, x, ldx, q, ldq, scale, rows, k);
+    if (vec && k <= 512) return run(quantize_rows_kernel<T, 32, 2>, 32, true, x, ldx, q, ldq, scale, rows, k);
+    if (vec && k <= 1024) return run(quantize_rows_kernel<T, 32, 4>, 32, true, x, ldx, q, ldq, scale, rows, k);
+    if (vec && k <= 2048) return run(quantize_rows_kernel<T, 128, 2>, 128, true, x, ldx, q, ldq, scale, rows, k);
+    if (vec && k <= 4096) return run(quantize_rows_kernel<T, 256, 2>, 256, true, x, ldx, q, ldq, scale, rows, k);
+    if (vec && k <= 8192) return run(quantize_rows_kernel<T, 256, 4>, 256, true, x, ldx, q, ldq, scale, rows, k);
+    if (vec && k <= 16384) return run(quantize_rows_kernel<T, 512, 4>, 512, true, x, ldx, q, ldq, scale, rows, k);
+    if (k <= 1024) return run(quantize_rows_any_kernel<T, 32>, 32, false, x, ldx, q, ldq, scale, rows, k);
+    if (k <= 4096) return run(quantize_rows_any_kernel<T, 128>, 128, false, x, ldx, q, ldq, scale, rows, k);
+    if (k <= 16384) return run(quantize_rows_any_kernel<T, 512>, 512, false, x, ldx, q, ldq, scale, rows, k);
+    return run(quantize_rows_long_kernel<T>, 512, false, x, ldx, q, ldq, scale, k);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -152,8 +222,11 @@ static int quantize_rows(const T* x, long ldx, int8_t* q, long ldq, float* scale
 //   warp 0      TMA producer, 128 bytes of K per stage (past K, M and N the tensor maps read zeros)
 //   warp 1      TMEM allocation; lane 0 issues the MMAs (32 bytes of K each) and commits
 //   warps 2..9  two epilogue sets of four warps (one per TMEM lane quadrant): set s takes the tiles of parity s
-// The result leaves by TMA stores where its rows start at multiples of 16 bytes, else in 64- or 128-byte pieces of
-// a row from a staging tile.
+// The result passes through a staging tile per warp, 128 bytes of a row at a time, so that every store writes whole
+// lines (35,328 x 4,096 x 512 to bf16: 102 us, 111 with TMA stores of 64-byte rows; writing alone runs at 3.9 TB/s).
+// Tiles are taken in panels of columns whose weights stay in L2 while the rows go by. Integer sums do not depend on
+// their order, so a single CTA begins its K range at a place of its own: weights with rows of a large power of two
+// bytes would otherwise be read at the same few memory channels by all CTAs at once.
 // ---------------------------------------------------------------------------------------------
 constexpr int I8_THREADS = 320;
 template <bool PAIR>
@@ -163,8 +236,8 @@ struct I8Cfg {
     static constexpr int B_BYTES = PAIR ? 128 * 128 : 64 * 128;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = PAIR ? 5 : 6;
-    static constexpr int OFF_OUT = STAGES * STAGE;          // per epilogue warp: two 2 KB slots
-    static constexpr int OFF_SC = OFF_OUT + 8 * 4096;       // per epilogue warp: the tile's scales and biases
+    static constexpr int OFF_OUT = STAGES * STAGE;          // per epilogue warp: 32 rows of 128 + 16 bytes
+    static constexpr int OFF_SC = OFF_OUT + 8 * 32 * 144;      // per epilogue warp: the tile's scales and biases
     static constexpr int OFF_BAR = OFF_SC + 8 * 8 * BN;
     static constexpr int N_BARS = 2 * STAGES + 5;
     static constexpr int SMEM = 1024 + OFF_BAR + N_BARS * 8 + 16;
@@ -190,27 +263,19 @@ EG2_DEV void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t id
             "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
-// int to float on the integer and FMA pipes, rounded once like the conversion instruction: x = 65536 h + l with both
-// halves placed in the mantissa of 2^23. The epilogue converts every other value this way, since the conversion unit alone
-// (16 a cycle) would take as long as the MMAs of a product over K = 512.
-EG2_DEV float i32_to_f32(uint32_t x) {
-    const float l = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7410)) - 8388608.f;
-    const float h = __uint_as_float(__byte_perm(x ^ 0x80000000u, 0x4b000000u, 0x7432)) - 8421376.f;  // 2^23 + 2^15
-    return fmaf(h, 65536.f, l);
-}
-
 struct I8Params {
     const float *sa, *sw, *bias;
     void* C;
     long ldc;
     int M, N, K;
-    int tma_out;
+    int panel;    // column tiles per panel of the tile order
+    int aligned;  // rows of C start at multiples of 16 bytes
 };
 
 template <bool PAIR, typename TO>
 __global__ void __launch_bounds__(I8_THREADS, 1)
     gemm_i8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
-                      const __grid_constant__ CUtensorMap tmC, const I8Params p) {
+                      const I8Params p) {
     using Cfg = I8Cfg<PAIR>;
     constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BM = PAIR ? 256 : 128;
     extern __shared__ uint8_t smem_raw[];
@@ -227,7 +292,14 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     const bool lead = rank == 0;
     const int tiles_n = (p.N + BN - 1) / BN, tiles = ((p.M + BM - 1) / BM) * tiles_n;
     const int t_first = (int)(blockIdx.x / (PAIR ? 2 : 1)), t_step = (int)(gridDim.x / (PAIR ? 2 : 1));
-    const int kblocks = (p.K + 127) / 128;
+    const int kblocks = (p.K + 127) / 128, tiles_m = (p.M + BM - 1) / BM;
+    // Tile t: panels of p.panel column tiles, rows within a panel, columns within a row.
+    auto place = [&](int t, int& m0, int& n0) {
+        const int per = tiles_m * p.panel, pan = t / per, left = t - pan * per;
+        const int width = min(p.panel, tiles_n - pan * p.panel);
+        m0 = (left / width) * BM + 128 * (int)rank;
+        n0 = (pan * p.panel + left % width) * BN;
+    };
 
     if (threadIdx.x == 0) {
         for (int x = 0; x < STAGES; x++) {
@@ -243,7 +315,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
         fence_mbarrier_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmW);
-        if (p.tma_out) tma_prefetch_desc(&tmC);
     }
     if (warp == 1) {
         if constexpr (PAIR)
@@ -264,8 +335,11 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
             int loads = 0;
             bool ok = true;
             for (int t = t_first; ok && t < tiles; t += t_step) {
-                const int m0 = (t / tiles_n) * BM + 128 * (int)rank, n0 = (t % tiles_n) * BN + (PAIR ? 128 * (int)rank : 0);
-                for (int kb = 0; kb < kblocks; kb++, loads++) {
+                int m0, n0;
+                place(t, m0, n0);
+                if (PAIR) n0 += 128 * (int)rank;
+                int kb = PAIR ? 0 : (int)((unsigned)(n0 / BN) * 13u % (unsigned)kblocks);
+                for (int i = 0; i < kblocks; i++, loads++, kb = kb + 1 == kblocks ? 0 : kb + 1) {
                     const int st = loads % STAGES;
                     if (!(ok = mbar_wait(&empty[st], ((loads / STAGES) & 1) ^ 1, EG2_DEV_TIMEOUT_GEMM, abort_flag))) break;
                     uint8_t* sa = smem + st * Cfg::STAGE;
@@ -318,12 +392,14 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
         }
     } else {
         const int w = warp - 2, set = w >> 2, e = warp & 3;
-        uint8_t* slots = smem + Cfg::OFF_OUT + w * 4096;
+        uint8_t* stage = smem + Cfg::OFF_OUT + w * 32 * 144;
         float* sc = reinterpret_cast<float*>(smem + Cfg::OFF_SC + w * 8 * BN);
-        int local = 0, nst = 0;
+        int local = 0;
         for (int t = t_first; t < tiles; t += t_step, local++) {
             if ((local & 1) != set) continue;
-            const int row0 = (t / tiles_n) * BM + 128 * (int)rank + 32 * e, n0 = (t % tiles_n) * BN;
+            int row0, n0;
+            place(t, row0, n0);
+            row0 += 32 * e;
             const int row = row0 + lane;
             // Scales and biases of the tile's columns, requested before the sums are there.
             const float sa = row < p.M ? p.sa[row] : 0.f;
@@ -338,55 +414,50 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
             tc_fence_after();
             const uint32_t base = tmem + set * BN + ((uint32_t)(32 * e) << 16);
             const int chunks = row0 < p.M ? min(BN / 32, (p.N - n0 + 31) / 32) : 0;
+            constexpr int COLS = 128 / (int)sizeof(TO);  // columns of a staged row: two chunks of bf16, one of f32
+            TO* out = (TO*)p.C + (long)row0 * p.ldc + n0;
+            const int rows = min(32, p.M - row0);
             auto chunk = [&](int c, uint32_t (&r)[32]) -> bool {
-                float v[32];
+                uint8_t* mine = stage + lane * 144 + (sizeof(TO) == 2 ? (c & 1) * 64 : 0);
 #pragma unroll
-                for (int q = 0; q < 32; q += 4) {
-                    const float4 s4 = *reinterpret_cast<const float4*>(sc + 32 * c + q), b4 = *reinterpret_cast<const float4*>(sc + BN + 32 * c + q);
-                    v[q] = fmaf((float)(int)r[q] * sa, s4.x, b4.x);
-                    v[q + 1] = fmaf(i32_to_f32(r[q + 1]) * sa, s4.y, b4.y);
-                    v[q + 2] = fmaf((float)(int)r[q + 2] * sa, s4.z, b4.z);
-                    v[q + 3] = fmaf(i32_to_f32(r[q + 3]) * sa, s4.w, b4.w);
-                }
-                if (p.tma_out) {
+                for (int q = 0; q < 32; q += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int y = 0; y < 8; y += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(sc + 32 * c + q + y);
+                        const float4 b4 = *reinterpret_cast<const float4*>(sc + BN + 32 * c + q + y);
+                        v[y] = fmaf((float)(int)r[q + y] * sa, s4.x, b4.x);
+                        v[y + 1] = fmaf((float)(int)r[q + y + 1] * sa, s4.y, b4.y);
+                        v[y + 2] = fmaf((float)(int)r[q + y + 2] * sa, s4.z, b4.z);
+                        v[y + 3] = fmaf((float)(int)r[q + y + 3] * sa, s4.w, b4.w);
+                    }
                     if constexpr (sizeof(TO) == 2) {
-                        tio_store32<2>(&tmC, slots, nst++, v, n0 + 32 * c, row0);
+                        *reinterpret_cast<uint4*>(mine + 2 * q) = make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]),
+                                                                             bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7]));
                     } else {
-                        // 16 columns per 2 KB slot, 64-byte swizzle.
-                        const uint32_t swz = (uint32_t)((lane >> 1) & 3);
+                        *reinterpret_cast<float4*>(mine + 4 * q) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4*>(mine + 4 * q + 16) = make_float4(v[4], v[5], v[6], v[7]);
+                    }
+                }
+                if (sizeof(TO) == 2 && !(c & 1) && c + 1 < chunks) return true;
+                __syncwarp();
+                const int first = sizeof(TO) == 2 ? 32 * (c & ~1) : 32 * c;  // the staged columns start here in the tile
+                const int width = min(p.N - n0 - first, COLS);
+                if (p.aligned && width == COLS && (sizeof(TO) == 4 || (c & 1))) {
+                    // 8 lanes a row, 4 rows an instruction: whole 128-byte pieces.
+                    const int at = (lane & 7) * 16;
 #pragma unroll
-                        for (int hh = 0; hh < 2; hh++, nst++) {
-                            uint8_t* slot = slots + (nst & 1) * 2048;
-                            if (lane == 0) bulk_wait_read<1>();
-                            __syncwarp();
-#pragma unroll
-                            for (int q = 0; q < 4; q++)
-                                *reinterpret_cast<float4*>(slot + lane * 64 + ((q ^ swz) << 4)) =
-                                    make_float4(v[16 * hh + 4 * q], v[16 * hh + 4 * q + 1], v[16 * hh + 4 * q + 2], v[16 * hh + 4 * q + 3]);
-                            fence_proxy_async();
-                            __syncwarp();
-                            if (lane == 0) {
-                                if (n0 + 32 * c + 16 * hh < p.N) tma_store_2d(&tmC, slot, n0 + 32 * c + 16 * hh, row0);
-                                bulk_commit();
-                            }
-                        }
+                    for (int y = 0; y < 8; y++) {
+                        const int rr = 4 * y + (lane >> 3);
+                        const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 144 + at);
+                        if (rr < rows) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + (long)rr * p.ldc + first) + at) = x;
                     }
                 } else {
-                    // 16 columns at a time through a padded tile, then lanes 0..15 and 16..31 write two rows' pieces.
-                    float* tile = reinterpret_cast<float*>(slots);  // [32][17]
-#pragma unroll
-                    for (int hh = 0; hh < 2; hh++) {
-#pragma unroll
-                        for (int q = 0; q < 16; q++) tile[lane * 17 + q] = v[16 * hh + q];
-                        __syncwarp();
-                        const int n = n0 + 32 * c + 16 * hh + (lane & 15);
-#pragma unroll 4
-                        for (int rr = lane >> 4; rr < 32; rr += 2)
-                            if (row0 + rr < p.M && n < p.N)
-                                stf((TO*)p.C + (long)(row0 + rr) * p.ldc, n, tile[rr * 17 + (lane & 15)]);
-                        __syncwarp();
-                    }
+                    for (int rr = 0; rr < rows; rr++)
+                        for (int y = lane; y < width; y += 32)
+                            out[(long)rr * p.ldc + first + y] = reinterpret_cast<const TO*>(stage + rr * 144)[y];
                 }
+                __syncwarp();
                 return true;
             };
             if (chunks > 0) tmem_pipelined<32>(base, chunks, chunk);
@@ -399,8 +470,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
                     mbar_arrive(&tempty[set]);
             }
         }
-        if (lane == 0) bulk_wait_all();
-        __syncwarp();
     }
     // Every MMA has completed before either CTA frees its TMEM.
     if (warp == 1 && lane == 0 && lead) {
@@ -423,7 +492,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
 }
 
 template <bool PAIR, typename TO>
-static int launch_i8(const int8_t* A, long lda, const int8_t* W, long ldw, const I8Params& p, cudaStream_t s) {
+static int launch_i8(const int8_t* A, long lda, const int8_t* W, long ldw, I8Params p, cudaStream_t s) {
     using Cfg = I8Cfg<PAIR>;
     auto kern = gemm_i8_tc_kernel<PAIR, TO>;
     static int clusters_max[64] = {0};
@@ -450,28 +519,26 @@ static int launch_i8(const int8_t* A, long lda, const int8_t* W, long ldw, const
         if (PAIR && (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0)) return -3;
         clusters_max[dev] = n;
     }
-    CUtensorMap ma, mw, mc;
+    CUtensorMap ma, mw;
     if (make_tmap_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, p.K, p.M, lda, 128, 128) ||
         make_tmap_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, W, p.K, p.N, ldw, 128, PAIR ? 128 : 64))
         return -1;
-    constexpr bool F32 = sizeof(TO) == 4;
-    mc = ma;  // unused without tma_out
-    if (p.tma_out && make_tmap_2d(&mc, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.C, p.N, p.M,
-                                  p.ldc * sizeof(TO), F32 ? 16 : 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
-        return -1;
     const long tiles = (((long)p.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128)) * ((p.N + Cfg::BN - 1) / Cfg::BN);
     if (tiles > 0x7fffffffL) return -1;
+    // 24 MB of weights per panel: a fifth of L2, which also holds the rows passing by.
+    const long per_panel = (24L << 20) / ((long)Cfg::BN * p.K);
+    p.panel = per_panel < 1 ? 1 : per_panel > 4096 ? 4096 : (int)per_panel;
     const int n = tiles < clusters_max[dev] ? (int)tiles : clusters_max[dev];
     cfg.gridDim = dim3((PAIR ? 2 : 1) * n, 1, 1);
     attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = n_attr + (pdl_enabled() ? 1 : 0);
-    return cudaLaunchKernelEx(&cfg, kern, ma, mw, mc, p) == cudaSuccess ? 0 : -3;
+    return cudaLaunchKernelEx(&cfg, kern, ma, mw, p) == cudaSuccess ? 0 : -3;
 }
 
 template <typename TO>
 static int gemm_i8(const int8_t* A, long lda, const int8_t* W, long ldw, I8Params& p, cudaStream_t s) {
-    p.tma_out = (uintptr_t)p.C % 16 == 0 && p.ldc * sizeof(TO) % 16 == 0;
+    p.aligned = (uintptr_t)p.C % 16 == 0 && p.ldc * sizeof(TO) % 16 == 0;
     // Pairs where their 256 x 256 tiles fill at least half of the SM pairs.
     const long pair_tiles = (((long)p.M + 255) / 256) * ((p.N + 255) / 256);
     return pair_tiles >= num_sms() / 4 ? launch_i8<true, TO>(A, lda, W, ldw, p, s) : launch_i8<false, TO>(A, lda, W, ldw, p, s);
@@ -499,7 +566,7 @@ int eg2_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t
     if (M < 0 || N <= 0 || K <= 0 || K > EG2_I8_MAX_K || lda < K || ldw < K || ldc < N || lda % 16 || ldw % 16) return EG2_ERR_INVALID;
     if (M == 0) return EG2_OK;
     if (!A || !W || !a_scale || !w_scale || !C || M > (1L << 30) || ((uintptr_t)A | (uintptr_t)W) % 16) return EG2_ERR_INVALID;
-    eg2::I8Params p{a_scale, w_scale, bias, C, ldc, (int)M, N, K, 0};
+    eg2::I8Params p{a_scale, w_scale, bias, C, ldc, (int)M, N, K, 0, 0};
     const int rc = out_f32 ? eg2::gemm_i8<float>(A, lda, W, ldw, p, (cudaStream_t)stream)
                            : eg2::gemm_i8<bf16_t>(A, lda, W, ldw, p, (cudaStream_t)stream);
     if (rc == -1) return EG2_ERR_INVALID;

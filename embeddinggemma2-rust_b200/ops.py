@@ -115,8 +115,8 @@ def rotary(q, k, pos, steps, *, layout: str = "half", rot_dim: int | None = None
         if k.shape[0] != rows or k.shape[2] != hd:
             _bad(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
     if out is None:
-        qo = torch.empty((rows, nh, hd), dtype=kind, device=q.device)
-        ko = None if k is None else torch.empty((rows, nkv, hd), dtype=kind, device=q.device)
+        qo = torch.empty(rows, nh, hd, dtype=kind, device=q.device)
+        ko = None if k is None else torch.empty(rows, nkv, hd, dtype=kind, device=q.device)
         ldqo, ldko = nh * hd, nkv * hd
     else:
         qo, ko = out
@@ -184,7 +184,7 @@ def attention_masked(q, k, v, q_off, k_off, max_q: int, max_k: int, *, scale: fl
         radius = dist_bias.shape[1] // 2
         tensors.append(dist_bias)
     if out is None:
-        out = torch.empty((q_rows, nh, hd), dtype=kind, device=q.device)
+        out = torch.empty(q_rows, nh, hd, dtype=kind, device=q.device)
         ldo = nh * hd
     else:
         ldo = _heads(out, "out", kind)
@@ -192,7 +192,7 @@ def attention_masked(q, k, v, q_off, k_off, max_q: int, max_k: int, *, scale: fl
             _bad("out does not match q")
         tensors.append(out)
     stream = _stream(*tensors)
-    lse = torch.empty((q_rows, nh), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty(q_rows, nh, dtype=torch.float32, device=q.device) if return_lse else None
 
     def ptr(t):
         return None if t is None else t.data_ptr()
@@ -225,7 +225,7 @@ def quantize_rows(x):
     if ldx < k:
         _bad(f"x: the rows overlap (strides {x.stride()})")
     ld = (k + 15) // 16 * 16
-    q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
+    q = torch.empty(rows, ld, dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     stream = _stream(x)
     if rows:
@@ -256,7 +256,7 @@ def gemm_i8(a, a_scale, w, w_scale, *, bias=None, out_dtype=torch.bfloat16, out=
     if out is None:
         if out_dtype not in KINDS:
             _bad(f"out_dtype {out_dtype}: bf16 or f32")
-        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        out = torch.empty(m, n, dtype=out_dtype, device=a.device)
         ldc = n
     else:
         if tuple(out.shape) != (m, n) or out.dtype not in KINDS or (n > 1 and out.stride(1) != 1):
