@@ -24,7 +24,8 @@ struct MaskedParams {
     const int *q_off, *k_off, *prefix, *q_doc, *k_doc;
     const float *slopes, *table;
     long q_rows, k_rows;
-    int n_seq, max_q, max_k, nh, nkv, hd, G, window, causal, radius, nsplit;
+    int n_seq, max_q, max_k, nh, nkv, hd, G, window, causal, radius;
+    int nsplit, part;  // the key axis in nsplit parts of `part` key tiles each
     float scale, softcap;
     float *part_o, *part_lse;  // nsplit > 1: [nsplit][q_rows][nh][hd] and [nsplit][q_rows][nh]
 };
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
         }
     }
     const int first = k_lo / 64, tiles = k_hi > k_lo ? (k_hi + 63) / 64 - first : 0;
-    const int j_first = first + (int)((long)tiles * split / p.nsplit), j_last = first + (int)((long)tiles * (split + 1) / p.nsplit);
+    const int j_first = first + min(tiles, split * p.part), j_last = min(first + tiles, j_first + p.part);
 
     float m[RPT], l[RPT], o[NCH][RPT][4];
 #pragma unroll
@@ -317,14 +318,16 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
 
 #include "attention_masked_tc.cuh"
 
-// Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. One warp per (row, head).
+// Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. A block per (row, head): the
+// weights once, in shared memory, then a thread per channel. Bound by latency: few rows, their parts read once.
 template <typename T>
-__global__ void attention_masked_join_kernel(const MaskedParams p) {
-    const long item = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (item >= p.q_rows * p.nh) return;
-    const int lane = threadIdx.x & 31;
-    const long row = item / p.nh, step = p.q_rows * p.nh;
-    const int h = (int)(item % p.nh);
+__global__ void __launch_bounds__(128) attention_masked_join_kernel(const MaskedParams p) {
+    extern __shared__ float weight[];  // [nsplit]
+    __shared__ float red[4];
+    grid_dep_launch();
+    grid_dep_wait();
+    const long item = blockIdx.x, row = item / p.nh, step = p.q_rows * p.nh;
+    const int h = (int)(item % p.nh), t = threadIdx.x;
     // Rows of no sequence were not computed: left alone.
     int b = 0, e = p.n_seq;
     while (b < e) {
@@ -334,20 +337,34 @@ __global__ void attention_masked_join_kernel(const MaskedParams p) {
     if (b >= p.n_seq) return;
     const MaskedSeq sq = masked_seq(p, b);
     if (row < sq.q0 || row >= sq.q0 + sq.nq) return;
-    float top = -INFINITY, total = 0.f;
-    for (int s = 0; s < p.nsplit; s++) top = fmaxf(top, p.part_lse[s * step + item]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int s = 0; s < p.nsplit; s++) total += expf(p.part_lse[s * step + item] - base);
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int c = lane; c < p.hd; c += 32) {
-        float a = 0.f;
-        for (int s = 0; s < p.nsplit; s++) {
-            const float w = expf(p.part_lse[s * step + item] - base) * inv;
-            if (w != 0.f) a = fmaf(w, p.part_o[(s * step + item) * p.hd + c], a);
-        }
-        stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, a);
+    float top = -INFINITY;
+    for (int s = t; s < p.nsplit; s += 128) {
+        weight[s] = p.part_lse[s * step + item];
+        top = fmaxf(top, weight[s]);
     }
-    if (lane == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((t & 31) == 0) red[t >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int s = t; s < p.nsplit; s += 128) weight[s] = expf(weight[s] - base);
+    __syncthreads();
+    float total = 0.f;
+    for (int s = 0; s < p.nsplit; s++) total += weight[s];  // the same sum in every thread
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    for (int c = t; c < p.hd; c += 128) {
+        const float* o = p.part_o + item * p.hd + c;
+        float a = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < p.nsplit; s++) {
+            const float w = weight[s];
+            const float x = w != 0.f ? o[s * step * p.hd] : 0.f;  // a part that counts nothing may hold anything
+            a = fmaf(w, x, a);
+        }
+        stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, a * inv);
+    }
+    if (t == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
 }
 
 template <typename T, int NCH, int RPT>
@@ -379,10 +396,19 @@ static int attention_masked_simt(const MaskedParams& p, int vec, cudaStream_t s)
 
 template <typename T>
 static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
-    const long blocks = (p.q_rows * p.nh + 3) / 4;
+    const long blocks = p.q_rows * p.nh;
     if (blocks > 0x7fffffffL) return -1;
-    attention_masked_join_kernel<T><<<(unsigned)blocks, 128, 0, s>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : -3;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.dynamicSmemBytes = p.nsplit * 4;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, attention_masked_join_kernel<T>, p) == cudaSuccess ? 0 : -3;
 }
 
 // How a call runs. The tensor cores take bf16 whose rows and heads TMA can address (16-byte multiples) and G query
@@ -390,7 +416,7 @@ static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
 // kept for them; the rest runs on the CUDA cores.
 struct MaskedPlan {
     bool tc;
-    int Gt, nsplit;
+    int Gt, nsplit, part;
 };
 static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     MaskedPlan r;
@@ -400,14 +426,19 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
            a->q_rows < (1L << 31) && a->k_rows < (1L << 31) - 128;
     r.Gt = G;
     if (r.tc && (128 % G || (a->dist_bias && G * (2L * a->dist_radius + 257) > AMT_TABLE))) r.Gt = 1;
-    // The key axis is split when the tiles alone leave most SMs idle: parts of at least 4 key tiles, at most one
-    // part per idle SM.
+    // The key axis is split into parts of a fixed number of key tiles when the query tiles alone leave SMs idle: about
+    // two parts per SM where all sequences are as long as the longest (fewer where not), so that short ones do not
+    // hold up long ones. A part pays for its partial result, 128 rows of it more than one: at least 8 tiles, or 2 where a
+    // query tile is mostly empty.
     const int rows = r.tc ? 128 : 64, keys = r.tc ? 128 : 64;
-    const long base = ((long)a->max_q * r.Gt + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * (r.tc && a->hd > 256 ? 2 : 1);
+    const long tile_rows = (long)a->max_q * r.Gt;
+    const long base = (tile_rows + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * (r.tc && a->hd > 256 ? 2 : 1);
     const long key_tiles = ((long)a->max_k + keys - 1) / keys;
-    long n = num_sms() / (base > 0 ? base : 1);
-    if (n > key_tiles / 4) n = key_tiles / 4;
-    r.nsplit = n < 1 ? 1 : (int)n;
+    long part = (base * key_tiles + 2 * num_sms() - 1) / (2 * num_sms());
+    const long least = tile_rows > rows / 4 ? 8 : 2;
+    if (part < least) part = least;
+    r.nsplit = base >= num_sms() || part >= key_tiles ? 1 : (int)((key_tiles + part - 1) / part);
+    r.part = r.nsplit > 1 ? (int)part : (int)key_tiles;
     return r;
 }
 
@@ -444,10 +475,11 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
     if (!a->q || !a->out || !a->q_off || !a->k_off || (a->k_rows > 0 && (!a->k || !a->v))) return EG2_ERR_INVALID;
     MaskedParams p{a->q, a->k, a->v, a->out, a->lse, a->ldq, a->ldk, a->ldv, a->ldo, a->q_off, a->k_off, a->prefix_len, a->q_doc,
                    a->k_doc, a->slopes, a->dist_bias, a->q_rows, a->k_rows, a->n_seq, a->max_q, a->max_k, a->nh, a->nkv, a->hd,
-                   a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, a->scale, a->softcap, nullptr, nullptr};
+                   a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, 0, a->scale, a->softcap, nullptr, nullptr};
     cudaStream_t s = (cudaStream_t)stream;
     const MaskedPlan plan = masked_plan(a);
     p.nsplit = plan.nsplit;
+    p.part = plan.part;
     if (p.nsplit > 1) {
         if (!workspace || workspace_bytes < eg2_attention_masked_workspace(a) || (uintptr_t)workspace % 16) return EG2_ERR_INVALID;
         p.part_o = (float*)workspace;

@@ -47,6 +47,7 @@ struct alignas(16) AmtUnit {
     int n, first;     // key tiles to visit; the first (without documents they are consecutive,
     int down;         // and the first `down` of them are visited backwards)
     int stop, scrub, retry;  // no further unit; clean every V tile; (set by the softmax) run again with scrub
+    int masked;       // (set by the softmax) some tile was masked
     int n_bad;       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
     int bad[64];
     uint32_t visit[AMT_MASK_WORDS], docs[AMT_MASK_WORDS];
@@ -57,6 +58,7 @@ struct AmtParams {
     int Gt;              // query heads packed into a tile (G or 1)
     int q_tiles, heads;  // tiles per sequence; K/V heads x (G / Gt)
     int n_units;
+    int out32;           // rows of out start at multiples of 32 bytes, heads are multiples of 16 channels
 };
 
 template <int HD>
@@ -70,19 +72,21 @@ struct AmtCfg {
     static constexpr int KU = HD / (64 * UCH), VU = DV / (64 * UCH);  // ring units per K / V tile
     static constexpr int RING = HD == 64 ? 4 : 2;         // units of the K ring, and of the V ring
     static constexpr int NS = HD <= 128 ? 3 : 2;          // S buffers
+    // The producer of head 512, whose rings hold a fraction of a tile, loads whichever of K and V has room (954 us against
+    // 1,254 for 8,192 tokens, 4 heads); elsewhere it waits in order: its polling took issue slots from the softmax (320 -> 350 us
+    // at head 128).
+    static constexpr bool POLL = HD == 512;
     static constexpr int T_O = 128 * NS;
     static constexpr int OC = DV / 2;                     // O columns per thread in the epilogue
     static constexpr int OFF_R = QBUF * QCH * 16384;
     static constexpr int OFF_V = OFF_R + RING * UNIT;
     static constexpr int OFF_UNIT = OFF_V + RING * UNIT;
-    static constexpr int OFF_DOC = OFF_UNIT + 2 * (int)sizeof(AmtUnit);
-    static constexpr int OFF_X = OFF_DOC + 8 * 512;       // running maxima [2][128]; (maximum, sum) [2][2 groups][128]
+    static constexpr int OFF_X = OFF_UNIT + 2 * (int)sizeof(AmtUnit);       // running maxima [2][128]; (maximum, sum) [2][2 groups][128]
     static constexpr int OFF_TAB = OFF_X + 1024 + 4096;
     static constexpr int OFF_BAR = OFF_TAB + AMT_TABLE * 4;
     static constexpr int N_BARS = 4 + 2 * QBUF + 4 * RING + 3 * NS + 1 + 8 + 4 + 2 + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + N_BARS * 8 + 16;
 };
-static_assert(sizeof(AmtUnit) % 16 == 0, "the staged document ids are read 16 bytes at a time");
 static_assert(AmtCfg<64>::SMEM <= 227 * 1024 && AmtCfg<128>::SMEM <= 227 * 1024 && AmtCfg<256>::SMEM <= 227 * 1024 &&
                   AmtCfg<512>::SMEM <= 227 * 1024,
               "masked attention: shared memory");
@@ -122,6 +126,15 @@ EG2_DEV void mbar_arrive_if(uint64_t* bar, bool pred) {
         "r"((int)pred)
         : "memory");
 }
+EG2_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 EG2_DEV float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -140,7 +153,7 @@ struct BitWalk {
     const uint32_t* w;
     int at;
     uint32_t cur;
-    EG2_DEV explicit BitWalk(const uint32_t* words) : w(words), at(0), cur(words[0]) {}
+    EG2_DEV explicit BitWalk(const uint32_t* words) : w(words), at(0), cur(words ? words[0] : 0u) {}
     EG2_DEV int next() {  // there is one
         while (!cur && at + 1 < AMT_MASK_WORDS) cur = w[++at];
         const int b = __ffs(cur) - 1;
@@ -154,6 +167,7 @@ struct TileWalk {
     BitWalk bits;
     bool sparse;
     int first, down, j;
+    EG2_DEV TileWalk() : bits(nullptr), sparse(false), first(0), down(0), j(0) {}
     EG2_DEV TileWalk(const AmtUnit& u, bool docs) : bits(u.visit), sparse(docs), first(u.first), down(u.down), j(0) {}
     EG2_DEV int next() {
         const int i = j++;
@@ -284,7 +298,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; x++) {
             mbar_init(&unit_full[x], 32);
-            mbar_init(&unit_empty[x], 11);  // TMA, both MMA issuers, 8 softmax warps
+            mbar_init(&unit_empty[x], Cfg::POLL ? 12 : 11);  // TMA (both of its walks), both MMA issuers, 8 softmax warps
             mbar_init(&t_bar[x], 8);
             mbar_init(&drain[x], 1);
         }
@@ -336,6 +350,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0 && lane == 0) {
             int k_loads = 0, v_loads = 0, q_loads = 0;
+            if constexpr (!Cfg::POLL) {
             bool ok = true;
             for (int i = 0; ok; i++) {
                 const AmtUnit* un = unit_at(i);
@@ -374,6 +389,88 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     }
                 }
                 mbar_arrive(&unit_empty[i & 1]);
+            }
+            } else {
+            // Two walks over the units, one loading Q and K, one V; a step does what there is room for, or nothing.
+            struct Side {
+                int i = 0, j = 0, x = 0, kt = 0;  // unit, tile, ring unit of the tile, key tile
+                bool q = false, done = false;     // Q is loaded; no further unit
+                AmtUnit* un = nullptr;
+                TileWalk walk;
+            } ks, vs;
+            // Steps into the next unit with tiles. True where it moved.
+            auto enter = [&](Side& d) -> bool {
+                if (!mbar_test(&unit_full[d.i & 1], (d.i >> 1) & 1)) return false;
+                AmtUnit* un = &units[d.i & 1];
+                if (un->stop) {
+                    d.done = true;
+                } else if (un->n == 0) {
+                    mbar_arrive(&unit_empty[d.i & 1]);
+                    d.i++;
+                } else {
+                    d.un = un;
+                    d.j = d.x = 0;
+                    d.q = false;
+                    d.walk = TileWalk(*un, p.q_doc != nullptr);
+                    d.kt = d.walk.next();
+                }
+                return true;
+            };
+            auto load = [&](Side& d, const CUtensorMap* m, uint64_t* full, uint64_t* empty, int off, int& loads, int per, int ch0) -> bool {
+                const int u = loads % RING;
+                if (!mbar_test(&empty[u], ((loads / RING) & 1) ^ 1)) return false;
+                mbar_arrive_expect_tx(&full[u], Cfg::UNIT);
+                for (int c = 0; c < Cfg::UCH; c++)
+                    tma_load_3d(smem + off + u * Cfg::UNIT + c * 16384, m, &full[u], ch0 + (d.x * Cfg::UCH + c) * 64, d.un->g,
+                                (int)d.un->sq.k0 + d.kt * 128);
+                loads++;
+                if (++d.x == per) {
+                    d.x = 0;
+                    if (++d.j == d.un->n) {
+                        mbar_arrive(&unit_empty[d.i & 1]);
+                        d.i++;
+                        d.un = nullptr;
+                    } else {
+                        d.kt = d.walk.next();
+                    }
+                }
+                return true;
+            };
+            uint64_t since = 0;
+            for (uint32_t idle = 0; !(ks.done && vs.done);) {
+                bool moved = false;
+                if (!ks.done) {
+                    if (!ks.un) {
+                        moved = enter(ks);
+                    } else if (!ks.q) {
+                        const int qb = q_loads % QBUF;
+                        if (mbar_test(&q_empty[qb], ((q_loads / QBUF) & 1) ^ 1)) {
+                            mbar_arrive_expect_tx(&q_full[qb], Cfg::QCH * 16384);
+                            for (int c = 0; c < Cfg::QCH; c++)
+                                tma_load_3d(smem + (qb * Cfg::QCH + c) * 16384, &tmQ, &q_full[qb], 64 * c, ks.un->head0, (int)(ks.un->sq.q0 + ks.un->t0));
+                            q_loads++;
+                            moved = ks.q = true;
+                        }
+                    } else {
+                        moved = load(ks, &tmK, k_full, k_empty, Cfg::OFF_R, k_loads, KU, 0);
+                    }
+                }
+                if (!vs.done) moved |= vs.un ? load(vs, &tmV, v_full, v_empty, Cfg::OFF_V, v_loads, VU, vs.un->half * 256) : enter(vs);
+                if (moved) {
+                    idle = 0;
+                    continue;
+                }
+                __nanosleep(40);  // the softmax warps of this scheduler have the use of its issue slots
+                if ((++idle & 63u) == 0u) {  // the bounded wait of mbar_wait
+                    const uint64_t now = globaltimer_ns();
+                    if (idle == 64u) since = now;
+                    if (*abort_flag || *(volatile int*)&eg2_dev_status != 0 || now - since > EG2_WAIT_LIMIT_NS) {
+                        if (!*abort_flag) eg2_record_error(EG2_DEV_TIMEOUT_ATTN);
+                        *abort_flag = 1;
+                        break;
+                    }
+                }
+            }
             }
             // Every load has landed before the CTA may end (on the error path too).
             for (int x = max(0, q_loads - QBUF); x < q_loads; x++) mbar_drain(&q_full[x % QBUF], (x / QBUF) & 1, 200000000ull);
@@ -483,7 +580,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         un.stop = !again && idle;
                         un.scrub = again;
                         un.retry = 0;
-                        un.n_bad = 0;
+                        un.n_bad = un.masked = 0;
                         if (!again) un.n = un.rows = 0;
                         if (!again && !idle) un.visit[0] = 0u;
                     }
@@ -581,7 +678,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     }
                     if (p.nsplit > 1) {
                         // This part's share of the tiles: the a-th to the z-th of them.
-                        const int a = (int)((long)n * split / p.nsplit), z = (int)((long)n * (split + 1) / p.nsplit);
+                        const int a = min(n, split * p.part), z = min(n, a + p.part);
                         int before = 0;
                         for (int w0 = 0; w0 < w_end; w0 += 32) {
                             const int w = w0 + lane;
@@ -615,7 +712,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     un.n = n;
                     un.first = first_tile;
                     un.down = min(max(down_to + 1 - first_tile, 0), n);
-                    un.stop = un.scrub = un.retry = un.n_bad = 0;
+                    un.stop = un.scrub = un.retry = un.masked = un.n_bad = 0;
                 }
                 __syncwarp();
                 mbar_arrive(&unit_full[i & 1]);
@@ -627,7 +724,6 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const int r = 32 * e + lane;
         const uint32_t lane_off = (uint32_t)(32 * e) << 16;
         constexpr int NC = 128;
-        int* my_docs = reinterpret_cast<int*>(smem + Cfg::OFF_DOC) + (warp - 4) * 128;
         float* xm = reinterpret_cast<float*>(smem + Cfg::OFF_X);  // [2][128]
         float* xe = xm + 256;                                     // [2][2 groups][128][2]
         float* table = reinterpret_cast<float*>(smem + Cfg::OFF_TAB);
@@ -688,22 +784,44 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 const int all_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
                 const int mine = (wg ^ T) & 1;  // this group's tiles: mine, mine + 2, ...
                 if (mine) walk.next();
+                // The next tile's first key, and of its document ids those of columns lane, 32 + lane, ...
+                int next_key = mine < n ? walk.next() * 128 : 0, ids[4];
+                auto fetch_ids = [&] {
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const int key = next_key + 32 * x + lane;
+                        ids[x] = p.q_doc && key < un->sq.nk ? p.k_doc[un->sq.k0 + key] : 0;
+                    }
+                };
+                if (mine < n) fetch_ids();
                 int buf = (T + mine) % NS, phase = ((T + mine) / NS) & 1;
                 for (int j = mine; j < n; j += 2) {
-                    const int tile = T + j, kbase = walk.next() * 128;
-                    if (j + 2 < n) walk.next();
+                    const int tile = T + j, kbase = next_key;
                     const uint32_t ts = tmem + 128 * buf + lane_off;
                     const bool sees = kbase < some_hi && kbase + NC > some_lo;
                     const bool docs = p.q_doc && ((un->docs[kbase >> 12] >> ((kbase >> 7) & 31)) & 1u);
                     const bool full = !docs && kbase >= all_lo && kbase + NC <= all_hi;
                     any_masked |= !full;
+                    uint32_t same[4] = {~0u, ~0u, ~0u, ~0u};  // columns of this row's document
                     if (docs && sees) {
+                        // The rows of a warp are of few documents, mostly one: a ballot per document and 32 columns.
+                        uint32_t left = __ballot_sync(0xffffffffu, lo < hi);
 #pragma unroll
-                        for (int x = 0; x < NC / 32; x++) {
-                            const int key = kbase + 32 * x + lane;
-                            my_docs[32 * x + lane] = key < un->sq.nk ? p.k_doc[un->sq.k0 + key] : 0;
+                        for (int x = 0; x < 4; x++) same[x] = 0u;
+                        while (left) {
+                            const int d = __shfl_sync(0xffffffffu, qdoc, __ffs(left) - 1);
+                            left &= ~__ballot_sync(0xffffffffu, qdoc == d);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                const uint32_t cols = __ballot_sync(0xffffffffu, ids[x] == d);
+                                if (qdoc == d) same[x] = cols;
+                            }
                         }
-                        __syncwarp();
+                    }
+                    if (j + 2 < n) {
+                        walk.next();
+                        next_key = walk.next() * 128;
+                        fetch_ids();
                     }
                     if (ok) ok = mbar_wait(&s_full[buf], phase, EG2_DEV_TIMEOUT_ATTN, abort_flag);
                     tc_fence_after();
@@ -783,20 +901,10 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                             for (int x = 0; x < NC; x += 32) {
                                 const int u = min(max(lo - kbase - x, 0), 32), z = min(max(hi - kbase - x, 0), 32);
                                 uint32_t seen = z > u ? (0xffffffffu >> (32 - z)) & (0xffffffffu << u) : 0u;
-                                if (docs) {
-                                    uint32_t same = 0;
-#pragma unroll
-                                    for (int c = 0; c < 32; c += 4) {
-                                        const int4 d = *reinterpret_cast<const int4*>(my_docs + x + c);
-                                        same |= (d.x == qdoc ? 1u : 0u) << c | (d.y == qdoc ? 2u : 0u) << c | (d.z == qdoc ? 4u : 0u) << c |
-                                                (d.w == qdoc ? 8u : 0u) << c;
-                                    }
-                                    seen &= same;
-                                }
+                                seen &= same[x / 32];
 #pragma unroll
                                 for (int c = 0; c < 32; c++) sv[x + c] = (seen >> c) & 1u ? sv[x + c] : -INFINITY;
                             }
-                            if (docs) __syncwarp();
                         }
                         float mx[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
@@ -882,6 +990,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             {
                 float* mine = xe + (((U & 1) * 2 + wg) * 128 + r) * 2;
                 float* other = xe + (((U & 1) * 2 + (wg ^ 1)) * 128 + r) * 2;
+                if (any_masked && lane == 0) *(volatile int*)&un->masked = 1;
                 mine[0] = m;
                 mine[1] = l;
                 __syncwarp();
@@ -912,7 +1021,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 }
                 const int ch0 = un->half * 256 + wg * Cfg::OC;
                 const uint32_t to = tmem + Cfg::T_O + wg * Cfg::OC + lane_off;
-                bool odd = false;  // some channel is not finite
+                const bool some = n > 0 && l != 0.f;
+                float odd = 0.f;  // stays 0 while all channels are finite
 #pragma unroll 1
                 for (int c = 0; c < Cfg::OC; c += 32) {
                     uint32_t o[32];
@@ -923,40 +1033,45 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     }
 #pragma unroll
                     for (int q = 0; q < 32; q++) {
-                        const float x = n > 0 && l != 0.f ? __uint_as_float(o[q]) * inv : 0.f;
-                        odd |= !(fabsf(x) < INFINITY);
+                        const float x = some ? __uint_as_float(o[q]) * inv : 0.f;
+                        odd = fmaf(x, 0.f, odd);
                         o[q] = __float_as_uint(x);
                     }
                     if (live) {
 #pragma unroll
-                        for (int q = 0; q < 32; q += 8) {
+                        for (int q = 0; q < 32; q += 16) {
                             const int ch = ch0 + c + q;
-                            if (ch < p.hd) {
-                                if (p.nsplit > 1) {
-                                    float4* to4 = reinterpret_cast<float4*>(p.part_o + at * p.hd + ch);
-                                    to4[0] = make_float4(__uint_as_float(o[q]), __uint_as_float(o[q + 1]), __uint_as_float(o[q + 2]),
-                                                         __uint_as_float(o[q + 3]));
-                                    to4[1] = make_float4(__uint_as_float(o[q + 4]), __uint_as_float(o[q + 5]), __uint_as_float(o[q + 6]),
-                                                         __uint_as_float(o[q + 7]));
-                                } else {
-                                    uint32_t pk[4];
+                            if (ch >= p.hd) break;
+                            if (p.nsplit > 1) {
+                                float* part = p.part_o + at * p.hd + ch;
 #pragma unroll
-                                    for (int y = 0; y < 4; y++)
-                                        pk[y] = bf16x2_bits(__uint_as_float(o[q + 2 * y]), __uint_as_float(o[q + 2 * y + 1]));
-                                    *reinterpret_cast<uint4*>((bf16_t*)p.out + row * p.ldo + (long)head * p.hd + ch) =
-                                        make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                                for (int y = 0; y < 16; y += 4)
+                                    if (ch + y < p.hd)
+                                        *reinterpret_cast<uint4*>(part + y) = make_uint4(o[q + y], o[q + y + 1], o[q + y + 2], o[q + y + 3]);
+                            } else {
+                                uint32_t pk[8];
+#pragma unroll
+                                for (int y = 0; y < 8; y++)
+                                    pk[y] = bf16x2_bits(__uint_as_float(o[q + 2 * y]), __uint_as_float(o[q + 2 * y + 1]));
+                                bf16_t* out = (bf16_t*)p.out + row * p.ldo + (long)head * p.hd + ch;
+                                if (ap.out32) {
+                                    st_global_v8(out, pk);
+                                } else {
+                                    *reinterpret_cast<uint4*>(out) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                                    if (ch + 8 < p.hd) *reinterpret_cast<uint4*>(out + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
                                 }
                             }
                         }
                     }
+                    __syncwarp();
                 }
                 if (n > 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(o_empty);
+                    mbar_arrive_if(o_empty, lane == 0);
                 }
                 if (!un->scrub) {
-                    if (__any_sync(0xffffffffu, live && odd && any_masked) && lane == 0) *(volatile int*)&un->retry = 1;
+                    if (__any_sync(0xffffffffu, live && odd != 0.f) && *(volatile int*)&un->masked && lane == 0) *(volatile int*)&un->retry = 1;
                 } else {
                     bool sees_bad = un->n_bad > AMT_BAD;
                     for (int x = 0; x < min(un->n_bad, AMT_BAD); x++) {
@@ -1008,6 +1123,7 @@ static int launch_masked_tc(const MaskedParams& p, int Gt, cudaStream_t s) {
     const long units = (long)ap.q_tiles * p.n_seq * ap.heads * Cfg::HALVES * p.nsplit;
     if (units > 0x3fffffffL) return -1;
     ap.n_units = (int)units;
+    ap.out32 = (uintptr_t)p.out % 32 == 0 && (p.ldo | p.hd) % 16 == 0;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
