@@ -16,7 +16,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT = HERE / "_lib" / "libeg2_b200.so"
 SOURCES = ["eg2_lib.cu", "common.cuh", "kernels.h", "json.h", "gemm_tc.cu", "simt.cu", "rowops.cu", "attention_tc.cu", "noalloc.cu", "probe.cu", "runtime.cu",
-           "rotary.cu", "attention_masked.cu", "attention_masked_tc.cuh", "gemm_i8.cu"]
+           "rotary.cu", "attention_masked.cu", "attention_masked_tc.cuh", "attention_masked_few.cuh", "gemm_i8.cu"]
 
 
 def nvcc() -> str:

@@ -317,6 +317,7 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
 }
 
 #include "attention_masked_tc.cuh"
+#include "attention_masked_few.cuh"
 
 // Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. A block per (row, head): the
 // weights once, in shared memory, then a thread per channel. Bound by latency: few rows, their parts read once.
@@ -413,9 +414,11 @@ static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
 
 // How a call runs. The tensor cores take bf16 whose rows and heads TMA can address (16-byte multiples) and G query
 // heads that divide a 128-row tile are packed into it, unless their bias tables together pass the shared memory
-// kept for them; the rest runs on the CUDA cores.
+// kept for them; the rest runs on the CUDA cores. Calls whose query tiles would be at most an eighth full -- 16 rows --
+// are bound by reading K and V and take the form made for that (8 queries, 4 heads over 2 of 256, up to 11,774 keys: 75 us in
+// 128-row tiles).
 struct MaskedPlan {
-    bool tc;
+    bool tc, few;
     int Gt, nsplit, part;
 };
 static MaskedPlan masked_plan(const eg2_masked_attention* a) {
@@ -426,19 +429,21 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
            a->q_rows < (1L << 31) && a->k_rows < (1L << 31) - 128;
     r.Gt = G;
     if (r.tc && (128 % G || (a->dist_bias && G * (2L * a->dist_radius + 257) > AMT_TABLE))) r.Gt = 1;
+    r.few = r.tc && (long)a->max_q * G <= 16;
+    if (r.few) r.Gt = G;
     // The key axis is split into parts of a fixed number of key tiles when the query tiles alone leave SMs idle: about
     // two parts per SM where all sequences are as long as the longest (fewer where not), so that short ones do not
     // hold up long ones. A part pays for its partial result, 128 rows of it more than one: at least 8 tiles, or 2 where a
     // query tile is mostly empty.
-    const int rows = r.tc ? 128 : 64, keys = r.tc ? 128 : 64;
+    const int rows = r.few ? 16 : r.tc ? 128 : 64, keys = r.few ? 16 : r.tc ? 128 : 64;
     const long tile_rows = (long)a->max_q * r.Gt;
     const long base = (tile_rows + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * (r.tc && a->hd > 256 ? 2 : 1);
     const long key_tiles = ((long)a->max_k + keys - 1) / keys;
     long part = (base * key_tiles + 2 * num_sms() - 1) / (2 * num_sms());
-    const long least = tile_rows > rows / 4 ? 8 : 2;
+    const long least = r.few ? 16 : tile_rows > rows / 4 ? 8 : 2;
     if (part < least) part = least;
     r.nsplit = base >= num_sms() || part >= key_tiles ? 1 : (int)((key_tiles + part - 1) / part);
-    r.part = r.nsplit > 1 ? (int)part : (int)key_tiles;
+    r.part = r.nsplit > 1 ? (int)part : (int)(key_tiles > 0 ? key_tiles : 1);
     return r;
 }
 
@@ -486,7 +491,10 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
         p.part_lse = p.part_o + (long)p.nsplit * p.q_rows * p.nh * p.hd;
     }
     int rc;
-    if (plan.tc) {
+    if (plan.few) {
+        rc = a->hd <= 64 ? launch_masked_few<64>(p, s) : a->hd <= 128 ? launch_masked_few<128>(p, s)
+             : a->hd <= 256 ? launch_masked_few<256>(p, s) : launch_masked_few<512>(p, s);
+    } else if (plan.tc) {
         rc = a->hd <= 64 ? launch_masked_tc<64>(p, plan.Gt, s) : a->hd <= 128 ? launch_masked_tc<128>(p, plan.Gt, s)
              : a->hd <= 256 ? launch_masked_tc<256>(p, plan.Gt, s) : launch_masked_tc<512>(p, plan.Gt, s);
     } else {
