@@ -319,53 +319,77 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
 #include "attention_masked_tc.cuh"
 #include "attention_masked_few.cuh"
 
-// Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. A block per (row, head): the
-// weights once, in shared memory, then a thread per channel. Bound by latency: few rows, their parts read once.
+// Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. A block per (sequence, query, head),
+// two groups of 128 threads that take every other part; the parts' results are on their way while the weights are
+// worked out. Bound by latency: few rows, their parts read once.
 template <typename T>
-__global__ void __launch_bounds__(128) attention_masked_join_kernel(const MaskedParams p) {
-    extern __shared__ float weight[];  // [nsplit]
-    __shared__ float red[4];
+__global__ void __launch_bounds__(256) attention_masked_join_kernel(const MaskedParams p) {
+    extern __shared__ float weight[];  // [nsplit], then [hd] of the second group
+    __shared__ float red[8];
     grid_dep_launch();
     grid_dep_wait();
-    const long item = blockIdx.x, row = item / p.nh, step = p.q_rows * p.nh;
-    const int h = (int)(item % p.nh), t = threadIdx.x;
-    // Rows of no sequence were not computed: left alone.
-    int b = 0, e = p.n_seq;
-    while (b < e) {
-        const int mid = (b + e) / 2;
-        if (p.q_off[mid + 1] <= row) b = mid + 1; else e = mid;
-    }
-    if (b >= p.n_seq) return;
+    long id = blockIdx.x;
+    const int h = (int)(id % p.nh);
+    id /= p.nh;
+    const int t = (int)(id % p.max_q), b = (int)(id / p.max_q);
     const MaskedSeq sq = masked_seq(p, b);
-    if (row < sq.q0 || row >= sq.q0 + sq.nq) return;
+    if (t >= sq.nq) return;
+    const long row = sq.q0 + t, item = row * p.nh + h, step = p.q_rows * p.nh;
+    const int group = threadIdx.x >> 7, c0 = threadIdx.x & 127;
+    constexpr int AHEAD = 16;  // parts on their way, of the thread's first channel
+    float early[AHEAD];
+#pragma unroll
+    for (int y = 0; y < AHEAD; y++) {
+        const int s = group + 2 * y;
+        early[y] = s < p.nsplit && c0 < p.hd ? p.part_o[(s * step + item) * p.hd + c0] : 0.f;
+    }
     float top = -INFINITY;
-    for (int s = t; s < p.nsplit; s += 128) {
+    for (int s = threadIdx.x; s < p.nsplit; s += 256) {
         weight[s] = p.part_lse[s * step + item];
         top = fmaxf(top, weight[s]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((t & 31) == 0) red[t >> 5] = top;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int x = 0; x < 8; x++) top = fmaxf(top, red[x]);
     const float base = top == -INFINITY ? 0.f : top;
-    for (int s = t; s < p.nsplit; s += 128) weight[s] = expf(weight[s] - base);
+    for (int s = threadIdx.x; s < p.nsplit; s += 256) weight[s] = expf(weight[s] - base);
     __syncthreads();
     float total = 0.f;
     for (int s = 0; s < p.nsplit; s++) total += weight[s];  // the same sum in every thread
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int c = t; c < p.hd; c += 128) {
-        const float* o = p.part_o + item * p.hd + c;
-        float a = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < p.nsplit; s++) {
-            const float w = weight[s];
-            const float x = w != 0.f ? o[s * step * p.hd] : 0.f;  // a part that counts nothing may hold anything
-            a = fmaf(w, x, a);
+    float* second = weight + p.nsplit;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};  // hd is at most 512
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        const int c = c0 + 128 * x;
+        if (c >= p.hd) break;
+        // A part that counts nothing may hold anything.
+        int s = group;
+        if (x == 0) {
+#pragma unroll
+            for (int y = 0; y < AHEAD; y++, s += 2)
+                if (s < p.nsplit && weight[s] != 0.f) sum[x] = fmaf(weight[s], early[y], sum[x]);
         }
-        stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, a * inv);
+#pragma unroll 8
+        for (; s < p.nsplit; s += 2) {
+            const float w = weight[s];
+            const float o = w != 0.f ? p.part_o[(s * step + item) * p.hd + c] : 0.f;
+            sum[x] = fmaf(w, o, sum[x]);
+        }
+        if (group) second[c] = sum[x];
     }
-    if (t == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const int c = c0 + 128 * x;
+            if (c < p.hd) stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, (sum[x] + second[c]) * inv);
+        }
+        if (c0 == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+    }
 }
 
 template <typename T, int NCH, int RPT>
@@ -397,15 +421,15 @@ static int attention_masked_simt(const MaskedParams& p, int vec, cudaStream_t s)
 
 template <typename T>
 static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
-    const long blocks = p.q_rows * p.nh;
+    const long blocks = (long)p.n_seq * p.max_q * p.nh;
     if (blocks > 0x7fffffffL) return -1;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)blocks, 1, 1);
-    cfg.blockDim = dim3(128, 1, 1);
-    cfg.dynamicSmemBytes = p.nsplit * 4;
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.dynamicSmemBytes = (p.nsplit + p.hd) * 4;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
@@ -431,18 +455,22 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     if (r.tc && (128 % G || (a->dist_bias && G * (2L * a->dist_radius + 257) > AMT_TABLE))) r.Gt = 1;
     r.few = r.tc && (long)a->max_q * G <= 16;
     if (r.few) r.Gt = G;
-    // The key axis is split into parts of a fixed number of key tiles when the query tiles alone leave SMs idle: about
-    // two parts per SM where all sequences are as long as the longest (fewer where not), so that short ones do not
-    // hold up long ones. A part pays for its partial result, 128 rows of it more than one: at least 8 tiles, or 2 where a
-    // query tile is mostly empty.
+    // The key axis is split into parts of a fixed number of key tiles when the query tiles alone leave SMs idle, so many that
+    // the parts of all sequences are resident at once: their count is at most the key tiles there are (k_rows) over the part,
+    // and one more per sequence and head. A part pays for its partial result, 128 rows of it more than one: at least 8 tiles,
+    // or 2 where a query tile is mostly empty, or 256 keys in the form for few rows.
     const int rows = r.few ? 16 : r.tc ? 128 : 64, keys = r.few ? 16 : r.tc ? 128 : 64;
+    const int halves = r.tc && a->hd > 256 ? 2 : 1;
     const long tile_rows = (long)a->max_q * r.Gt;
-    const long base = (tile_rows + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * (r.tc && a->hd > 256 ? 2 : 1);
+    const long base = (tile_rows + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * halves;
     const long key_tiles = ((long)a->max_k + keys - 1) / keys;
-    long part = (base * key_tiles + 2 * num_sms() - 1) / (2 * num_sms());
+    const long slots = num_sms() * (r.few && halves == 1 ? 2L : 1L);
+    long all = base * key_tiles;
+    if (a->n_seq > 0 && base / a->n_seq * ((a->k_rows + keys - 1) / keys + a->n_seq) < all) all = base / a->n_seq * ((a->k_rows + keys - 1) / keys + a->n_seq);
+    long part = base < slots ? (all + slots - base - 1) / (slots - base) : key_tiles;
     const long least = r.few ? 16 : tile_rows > rows / 4 ? 8 : 2;
     if (part < least) part = least;
-    r.nsplit = base >= num_sms() || part >= key_tiles ? 1 : (int)((key_tiles + part - 1) / part);
+    r.nsplit = base >= slots || part >= key_tiles ? 1 : (int)((key_tiles + part - 1) / part);
     r.part = r.nsplit > 1 ? (int)part : (int)(key_tiles > 0 ? key_tiles : 1);
     return r;
 }

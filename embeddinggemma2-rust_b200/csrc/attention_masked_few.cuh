@@ -13,13 +13,13 @@
 template <int HD>
 struct AmfCfg {
     static constexpr int DV = HD < 256 ? HD : 256, HALVES = HD / DV;
-    static constexpr int WARPS = HD <= 128 ? 8 : 4;
-    static constexpr int STAGES = HD == 64 ? 6 : HD == 512 ? 2 : 3;
-    static constexpr int K_BYTES = 16 * HD * 2, STAGE = 16 * (HD + DV) * 2;
+    static constexpr int WARPS = 4, CTAS = HD == 512 ? 1 : 2;  // CTAs per SM
+    // Slots of 16 keys per warp; two CTAs of an SM then have about 128 KB under way.
+    static constexpr int KS = HD == 64 ? 6 : HD == 128 ? 3 : 2, VS = HD == 256 ? 1 : KS;
+    static constexpr int K_BYTES = 16 * HD * 2, V_BYTES = 16 * DV * 2, RING = KS * K_BYTES + VS * V_BYTES;
     static constexpr int OFF_RING = 16 * HD * 2;  // after Q
-    static constexpr int OFF_BAR = OFF_RING + WARPS * STAGES * STAGE;
-    static constexpr int OFF_BLOCKS = OFF_BAR + WARPS * STAGES * 8;  // bit mask of the part's blocks
-    static constexpr int MAX_WORDS = EG2_MASKED_MAX_LEN / 16 / 32;
+    static constexpr int OFF_BAR = OFF_RING + WARPS * RING;
+    static constexpr int OFF_BLOCKS = OFF_BAR + WARPS * (KS + VS) * 8;  // bit mask of the part's blocks
     static constexpr int SMEM = 1024 + OFF_BLOCKS;  // + the mask of the call's part
 };
 
@@ -46,16 +46,23 @@ EG2_DEV uint32_t amf_at(int row, int ch) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
+__global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
     attention_masked_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                 const __grid_constant__ MaskedParams p) {
     using Cfg = AmfCfg<HD>;
-    constexpr int DV = Cfg::DV, WARPS = Cfg::WARPS, STAGES = Cfg::STAGES;
+    constexpr int DV = Cfg::DV, WARPS = Cfg::WARPS, KS = Cfg::KS, VS = Cfg::VS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
     uint32_t* blocks = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BLOCKS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < WARPS * (KS + VS); x++) mbar_init(&bars[x], 1);
+        fence_mbarrier_init();
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+    }
+    __syncthreads();
     grid_dep_launch();
     grid_dep_wait();
     int id = blockIdx.x;
@@ -74,34 +81,9 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
     const int first = min(all_last, all_first + split * p.part), last = min(all_last, first + p.part);
     const int words = (last - first + 31) / 32;
 
-    // This thread's rows r0 and r0 + 8, and its columns of a block: 2 (lane % 4) + {0, 1} and 8 more.
-    int lo[2], hi[2], place[2], qdoc[2], head[2];
-    float slope[2];
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int r = (lane >> 2) + 8 * x, t = r < rows ? r / p.G : 0;
-        place[x] = sq.nk - sq.nq + t;
-        head[x] = g * p.G + r % p.G;
-        masked_range(p, sq, place[x], lo[x], hi[x]);
-        if (r >= rows) lo[x] = hi[x] = 0;
-        qdoc[x] = p.q_doc ? p.q_doc[sq.q0 + t] : 0;
-        slope[x] = p.slopes ? p.slopes[head[x]] * AMT_LOG2E : 0.f;
-    }
-    if (threadIdx.x == 0) {
-        for (int x = 0; x < WARPS * STAGES; x++) mbar_init(&bars[x], 1);
-        fence_mbarrier_init();
-        tma_prefetch_desc(&tmK);
-        tma_prefetch_desc(&tmV);
-    }
-    for (int w = threadIdx.x; w < words; w += blockDim.x) blocks[w] = p.q_doc ? 0u : w + 1 < words || !((last - first) & 31) ? ~0u : (1u << ((last - first) & 31)) - 1u;
-    for (int x = threadIdx.x; x < 16 * HD / 8; x += blockDim.x) {
-        const int r = x / (HD / 8), c = x % (HD / 8) * 8;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows && c < p.hd)
-            v = *reinterpret_cast<const uint4*>((const bf16_t*)p.q + (sq.q0 + r / p.G) * p.ldq + (long)(g * p.G + r % p.G) * p.hd + c);
-        *reinterpret_cast<uint4*>(smem + amf_at(r, c)) = v;
-    }
-    __syncthreads();
+    if (p.q_doc)
+        for (int w = threadIdx.x; w < words; w += blockDim.x) blocks[w] = 0u;
+    if (p.q_doc) __syncthreads();
     if (p.q_doc) {
         // Blocks with a key of some query's document (of their range of ids: the rows mask exactly).
         int dlo = INT_MAX, dhi = INT_MIN;
@@ -119,45 +101,87 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
         }
         __syncthreads();
     }
-    // This warp takes every WARPS-th of the marked blocks, the warp-th first.
-    int at_word = 0;
-    uint32_t left = words ? blocks[0] : 0u;
-    auto next_block = [&]() -> int {  // -1: none
-        while (!left) {
-            if (++at_word >= words) return -1;
-            left = blocks[at_word];
+    // This warp takes every WARPS-th block, with documents of the marked ones, the warp-th first. -1: none is left.
+    int at_word = 0, at_block = first + warp - WARPS;
+    uint32_t left = p.q_doc && words ? blocks[0] : 0u;
+    auto next_block = [&](int skip) -> int {
+        if (!p.q_doc) {
+            at_block += WARPS;
+            return at_block < last ? at_block : -1;
         }
-        const int bit = __ffs(left) - 1;
-        left &= left - 1u;
-        return first + at_word * 32 + bit;
+        for (; words; skip--) {
+            while (!left) {
+                if (++at_word >= words) return -1;
+                left = blocks[at_word];
+            }
+            const int bit = __ffs(left) - 1;
+            left &= left - 1u;
+            if (!skip) return first + at_word * 32 + bit;
+        }
+        return -1;
     };
-    auto my_next = [&](int skip) -> int {
-        int blk = words ? next_block() : -1;
-        for (int x = 0; x < skip && blk >= 0; x++) blk = next_block();
+    uint8_t* k_ring = smem + Cfg::OFF_RING + warp * Cfg::RING;
+    uint8_t* v_ring = k_ring + KS * Cfg::K_BYTES;
+    uint64_t* k_full = bars + warp * (KS + VS);
+    uint64_t* v_full = k_full + KS;
+    int queue[KS], k_issued = 0, v_issued = 0;  // the warp's n-th block, at n % KS
+    auto issue_k = [&](int blk) {
+        const int st = k_issued % KS;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&k_full[st], Cfg::K_BYTES);
+            for (int c = 0; c < HD / 64; c++) tma_load_3d(k_ring + st * Cfg::K_BYTES + c * 2048, &tmK, &k_full[st], 64 * c, g, (int)sq.k0 + blk * 16);
+        }
+        k_issued++;
+    };
+    auto issue_v = [&](int blk) {
+        const int st = v_issued % VS;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&v_full[st], Cfg::V_BYTES);
+            for (int c = 0; c < DV / 64; c++)
+                tma_load_3d(v_ring + st * Cfg::V_BYTES + c * 2048, &tmV, &v_full[st], half * 256 + 64 * c, g, (int)sq.k0 + blk * 16);
+        }
+        v_issued++;
+    };
+    auto queued = [&](int n) -> int {
+        int blk = queue[0];
+#pragma unroll
+        for (int x = 1; x < KS; x++)
+            if (n % KS == x) blk = queue[x];
         return blk;
     };
-    uint8_t* ring = smem + Cfg::OFF_RING + warp * STAGES * Cfg::STAGE;
-    uint64_t* full = bars + warp * STAGES;
-    int queue[STAGES], issued = 0;  // the blocks under way, by stage
-    auto issue = [&](int blk) {
-        const int st = issued % STAGES;
-        if (lane == 0) {
-            mbar_arrive_expect_tx(&full[st], Cfg::STAGE);
-            for (int c = 0; c < HD / 64; c++) tma_load_3d(ring + st * Cfg::STAGE + c * 2048, &tmK, &full[st], 64 * c, g, (int)sq.k0 + blk * 16);
-            for (int c = 0; c < DV / 64; c++)
-                tma_load_3d(ring + st * Cfg::STAGE + Cfg::K_BYTES + c * 2048, &tmV, &full[st], half * 256 + 64 * c, g, (int)sq.k0 + blk * 16);
-        }
-        issued++;
-    };
-    int blk = my_next(warp);
+    int blk = next_block(warp);
 #pragma unroll
-    for (int st = 0; st < STAGES; st++) {
+    for (int st = 0; st < KS; st++) {
         queue[st] = blk;
         if (blk >= 0) {
-            issue(blk);
-            blk = my_next(WARPS - 1);
+            issue_k(blk);
+            if (st < VS) issue_v(blk);
+            blk = next_block(WARPS - 1);
         }
     }
+
+    // This thread's rows r0 and r0 + 8, and its columns of a block: 2 (lane % 4) + {0, 1} and 8 more.
+    int lo[2], hi[2], place[2], qdoc[2], head[2];
+    float slope[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int r = (lane >> 2) + 8 * x, t = r < rows ? r / p.G : 0;
+        place[x] = sq.nk - sq.nq + t;
+        head[x] = g * p.G + r % p.G;
+        masked_range(p, sq, place[x], lo[x], hi[x]);
+        if (r >= rows) lo[x] = hi[x] = 0;
+        qdoc[x] = p.q_doc ? p.q_doc[sq.q0 + t] : 0;
+        slope[x] = p.slopes ? p.slopes[head[x]] * AMT_LOG2E : 0.f;
+    }
+    // Q, while the first blocks are under way.
+    for (int x = threadIdx.x; x < 16 * HD / 8; x += blockDim.x) {
+        const int r = x / (HD / 8), c = x % (HD / 8) * 8;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows && c < p.hd)
+            v = *reinterpret_cast<const uint4*>((const bf16_t*)p.q + (sq.q0 + r / p.G) * p.ldq + (long)(g * p.G + r % p.G) * p.hd + c);
+        *reinterpret_cast<uint4*>(smem + amf_at(r, c)) = v;
+    }
+    __syncthreads();
 
     const bool capped = p.softcap > 0.f;
     const float in_scale = capped ? p.scale / p.softcap : p.scale * AMT_LOG2E, cap2 = p.softcap * AMT_LOG2E;
@@ -167,55 +191,95 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
     for (int c = 0; c < DV / 8; c++)
 #pragma unroll
         for (int x = 0; x < 4; x++) o[c][x] = 0.f;
+    // ldmatrix addresses within a 64-channel chunk, by step of 16 channels: Q and V take rows (or keys) 0-7 / 8-15 by bit 3 of the
+    // lane and channels 0-7 / 8-15 by bit 4, K the other way round.
+    uint32_t q_off[4], k_off[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        q_off[c] = amf_at((lane & 7) + 8 * ((lane >> 3) & 1), 16 * c + 8 * (lane >> 4));
+        k_off[c] = amf_at((lane & 7) + 8 * (lane >> 4), 16 * c + 8 * ((lane >> 3) & 1));
+    }
     const uint32_t q_addr = smem_u32(smem);
+    // Keys that every row sees.
+    int all_lo = 0, all_hi = sq.nk;
+    masked_range(p, sq, sq.nk - 1, all_lo, tmp);
+    masked_range(p, sq, sq.nk - sq.nq, tmp, all_hi);
     bool ok = true;
     int taken = 0;
     while (true) {
-        const int st = taken % STAGES;
-        int now = queue[0];
-#pragma unroll
-        for (int x = 1; x < STAGES; x++)
-            if (st == x) now = queue[x];
+        const int now = queued(taken);
         if (now < 0) break;
         const int key0 = now * 16;
         // Document ids of this thread's four columns, under the latency of the block.
-        int ids[4];
+        int ids[4] = {0, 0, 0, 0};
+        if (p.k_doc) {
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            const int key = key0 + 8 * (x >> 1) + 2 * (lane & 3) + (x & 1);
-            ids[x] = p.k_doc && key < sq.nk ? p.k_doc[sq.k0 + key] : 0;
+            for (int x = 0; x < 4; x++) {
+                const int key = key0 + 8 * (x >> 1) + 2 * (lane & 3) + (x & 1);
+                ids[x] = key < sq.nk ? p.k_doc[sq.k0 + key] : 0;
+            }
         }
-        if (!(ok = mbar_wait(&full[st], (taken / STAGES) & 1, EG2_DEV_TIMEOUT_ATTN, nullptr))) break;
-        uint8_t* kb = ring + st * Cfg::STAGE;
-        uint8_t* vb = kb + Cfg::K_BYTES;
-        const uint32_t k_addr = smem_u32(kb), v_addr = smem_u32(vb);
+        if (!(ok = mbar_wait(&k_full[taken % KS], (taken / KS) & 1, EG2_DEV_TIMEOUT_ATTN, nullptr))) break;
+        const uint32_t k_addr = smem_u32(k_ring + (taken % KS) * Cfg::K_BYTES);
+        uint8_t* vb = v_ring + (taken % VS) * Cfg::V_BYTES;
+        const uint32_t v_addr = smem_u32(vb);
         float s[2][4] = {};
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD / 64; c0++) {
+            // Four steps of 16 channels: their eight loads are under way together.
+            uint32_t qa[4][4], kf[4][4];
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++) {
-            uint32_t qa[4], kf[4];
-            // Q: rows 0-7 / 8-15 x channels 0-7, then the same x channels 8-15; K: keys 0-7 x both, keys 8-15 x both.
-            ldmatrix4(q_addr + amf_at((lane & 7) + 8 * ((lane >> 3) & 1), 16 * c + 8 * (lane >> 4)), qa);
-            ldmatrix4(k_addr + amf_at((lane & 7) + 8 * (lane >> 4), 16 * c + 8 * ((lane >> 3) & 1)), kf);
-            mma_16816(s[0], qa, kf[0], kf[1]);
-            mma_16816(s[1], qa, kf[2], kf[3]);
+            for (int c = 0; c < 4; c++) {
+                ldmatrix4(q_addr + c0 * 2048 + q_off[c], qa[c]);
+                ldmatrix4(k_addr + c0 * 2048 + k_off[c], kf[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                mma_16816(s[0], qa[c], kf[c][0], kf[c][1]);
+                mma_16816(s[1], qa[c], kf[c][2], kf[c][3]);
+            }
+        }
+        __syncwarp();  // the K slot has been read
+#pragma unroll
+        for (int x = 0; x < KS; x++)
+            if (taken % KS == x) queue[x] = blk;
+        if (blk >= 0) {
+            issue_k(blk);
+            blk = next_block(WARPS - 1);
+        }
+        // Scores in the log2 domain: s[y / 2][2 x + y % 2] is row x, column y of this thread's.
+        float v[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) v[x] = s[(x >> 1) & 1][2 * (x >> 2) + (x & 1)] * in_scale;
+        if (capped) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] = cap2 * tanh_any(v[x]);
+        }
+        const int col0 = key0 + 2 * (lane & 3);
+        if (p.slopes) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] = fmaf(-slope[x >> 2], fabsf((float)(col0 + 8 * ((x >> 1) & 1) + (x & 1) - place[x >> 2])), v[x]);
+        }
+        if (p.table) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const int apart = col0 + 8 * ((x >> 1) & 1) + (x & 1) - place[x >> 2];
+                v[x] += masked_bias(p.table[(long)head[x >> 2] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]) * AMT_LOG2E;
+            }
         }
         bool hidden = false;  // some key is hidden from some row of this thread
-        float top[2] = {AMT_NONE, AMT_NONE};
+        if (p.k_doc || key0 < all_lo || key0 + 16 > all_hi) {
 #pragma unroll
-        for (int x = 0; x < 2; x++)  // row
-#pragma unroll
-            for (int y = 0; y < 4; y++) {  // column
-                float& v = s[y >> 1][2 * x + (y & 1)];
-                const int key = key0 + 8 * (y >> 1) + 2 * (lane & 3) + (y & 1), apart = key - place[x];
-                v = capped ? cap2 * tanh_any(v * in_scale) : v * in_scale;
-                if (p.slopes) v = fmaf(-slope[x], fabsf((float)apart), v);
-                if (p.table)
-                    v += masked_bias(p.table[(long)head[x] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]) * AMT_LOG2E;
-                const bool seen = key >= lo[x] && key < hi[x] && (!p.k_doc || ids[y] == qdoc[x]);
-                hidden |= !seen && (lane >> 2) + 8 * x < rows;
-                v = seen ? v : -INFINITY;
-                top[x] = fmaxf(top[x], v);
+            for (int x = 0; x < 8; x++) {
+                const int key = col0 + 8 * ((x >> 1) & 1) + (x & 1), y = x >> 2;
+                const bool seen = key >= lo[y] && key < hi[y] && (!p.k_doc || ids[x & 3] == qdoc[y]);
+                hidden |= !seen && (lane >> 2) + 8 * y < rows;
+                v[x] = seen ? v[x] : -INFINITY;
             }
+        }
+        float top[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) top[x] = fmaxf(fmaxf(fmaxf(v[4 * x], v[4 * x + 1]), fmaxf(v[4 * x + 2], v[4 * x + 3])), AMT_NONE);
         float factor[2];
         uint32_t pa[4];
 #pragma unroll
@@ -228,12 +292,11 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
             l[x] *= factor[x];
 #pragma unroll
             for (int y = 0; y < 4; y++) {
-                float& v = s[y >> 1][2 * x + (y & 1)];
-                v = ex2_approx(v - mn);
-                l[x] += v;
+                v[4 * x + y] = ex2_approx(v[4 * x + y] - mn);
+                l[x] += v[4 * x + y];
             }
-            pa[x] = bf16x2_bits(s[0][2 * x], s[0][2 * x + 1]);
-            pa[2 + x] = bf16x2_bits(s[1][2 * x], s[1][2 * x + 1]);
+            pa[x] = bf16x2_bits(v[4 * x], v[4 * x + 1]);
+            pa[2 + x] = bf16x2_bits(v[4 * x + 2], v[4 * x + 3]);
         }
         if (__any_sync(0xffffffffu, factor[0] != 1.f || factor[1] != 1.f)) {
 #pragma unroll
@@ -244,14 +307,15 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
                 o[c][3] *= factor[1];
             }
         }
+        if (!(ok = mbar_wait(&v_full[taken % VS], (taken / VS) & 1, EG2_DEV_TIMEOUT_ATTN, nullptr))) break;
         if (__any_sync(0xffffffffu, hidden)) {
             // A hidden key's value may be anything, and 0 x NaN must not reach the sum: elements that are not finite become
             // zero, after the rows that do see the key have taken them.
             uint32_t bad = 0;  // keys
             for (int x = lane; x < 16 * DV / 8; x += 32) {
                 const int key = x / (DV / 8), c = x % (DV / 8) * 8;
-                const uint4 v = *reinterpret_cast<const uint4*>(vb + amf_at(key, c));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                const uint4 e = *reinterpret_cast<const uint4*>(vb + amf_at(key, c));
+                const uint32_t w[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
                 for (int y = 0; y < 4; y++)
                     if ((w[y] & 0x7f80u) == 0x7f80u || (w[y] & 0x7f800000u) == 0x7f800000u) bad |= 1u << key;
@@ -260,49 +324,52 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
             for (; bad; bad &= bad - 1u) {
                 const int key = __ffs(bad) - 1;
                 const int src = (lane & ~3) + ((key & 7) >> 1);  // who holds this key's weights of my rows
-                const float a0 = __shfl_sync(0xffffffffu, s[0][key & 1 ? 1 : 0], src), a1 = __shfl_sync(0xffffffffu, s[0][key & 1 ? 3 : 2], src);
-                const float b0 = __shfl_sync(0xffffffffu, s[1][key & 1 ? 1 : 0], src), b1 = __shfl_sync(0xffffffffu, s[1][key & 1 ? 3 : 2], src);
-                const float w0 = key < 8 ? a0 : b0, w1 = key < 8 ? a1 : b1;
+                float w0 = 0.f, w1 = 0.f;
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const float a0 = __shfl_sync(0xffffffffu, v[y], src), a1 = __shfl_sync(0xffffffffu, v[4 + y], src);
+                    if (y == 2 * (key >> 3) + (key & 1)) w0 = a0, w1 = a1;
+                }
 #pragma unroll
                 for (int c = 0; c < DV / 8; c++)
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
-                        const float v = bf16_to_f32(*reinterpret_cast<const bf16_t*>(vb + amf_at(key, 8 * c + 2 * (lane & 3) + y)));
-                        if (!(fabsf(v) < INFINITY)) {
-                            if (w0 != 0.f) o[c][y] = fmaf(w0, v, o[c][y]);
-                            if (w1 != 0.f) o[c][2 + y] = fmaf(w1, v, o[c][2 + y]);
+                        const float e = bf16_to_f32(*reinterpret_cast<const bf16_t*>(vb + amf_at(key, 8 * c + 2 * (lane & 3) + y)));
+                        if (!(fabsf(e) < INFINITY)) {
+                            if (w0 != 0.f) o[c][y] = fmaf(w0, e, o[c][y]);
+                            if (w1 != 0.f) o[c][2 + y] = fmaf(w1, e, o[c][2 + y]);
                         }
                     }
                 __syncwarp();
                 for (int c = lane; c < DV; c += 32) {
-                    bf16_t* v = reinterpret_cast<bf16_t*>(vb + amf_at(key, c));
-                    if ((*v & 0x7f80u) == 0x7f80u) *v = 0;
+                    bf16_t* e = reinterpret_cast<bf16_t*>(vb + amf_at(key, c));
+                    if ((*e & 0x7f80u) == 0x7f80u) *e = 0;
                 }
                 __syncwarp();
             }
         }
 #pragma unroll
-        for (int c = 0; c < DV / 16; c++) {
-            uint32_t vf[4];
-            // V transposed: keys 0-7 and 8-15 x channels 0-7, then x channels 8-15.
-            ldmatrix4_trans(v_addr + amf_at((lane & 7) + 8 * ((lane >> 3) & 1), 16 * c + 8 * (lane >> 4)), vf);
-            mma_16816(o[2 * c], pa, vf[0], vf[1]);
-            mma_16816(o[2 * c + 1], pa, vf[2], vf[3]);
+        for (int c0 = 0; c0 < DV / 64; c0++) {
+            uint32_t vf[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) ldmatrix4_trans(v_addr + c0 * 2048 + q_off[c], vf[c]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                mma_16816(o[8 * c0 + 2 * c], pa, vf[c][0], vf[c][1]);
+                mma_16816(o[8 * c0 + 2 * c + 1], pa, vf[c][2], vf[c][3]);
+            }
         }
         fence_proxy_async();  // the cleaning's writes come before the next load's
-        __syncwarp();         // the stage has been read
+        __syncwarp();         // the V slot has been read
+        const int then = queued(taken + VS);
         taken++;
-#pragma unroll
-        for (int x = 0; x < STAGES; x++)
-            if (st == x) queue[x] = blk;
-        if (blk >= 0) {
-            issue(blk);
-            blk = my_next(WARPS - 1);
-        }
+        if (then >= 0) issue_v(then);
     }
     // No load may land after the CTA has ended (on the error path; else all have been waited for).
-    if (!ok && lane == 0)
-        for (int x = taken; x < issued; x++) mbar_drain(&full[x % STAGES], (x / STAGES) & 1, 200000000ull);
+    if (!ok && lane == 0) {
+        for (int x = max(0, k_issued - KS); x < k_issued; x++) mbar_drain(&k_full[x % KS], (x / KS) & 1, 200000000ull);
+        for (int x = max(0, v_issued - VS); x < v_issued; x++) mbar_drain(&v_full[x % VS], (x / VS) & 1, 200000000ull);
+    }
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
@@ -312,7 +379,7 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, 1)
     __syncthreads();
     float* mo = reinterpret_cast<float*>(smem + Cfg::OFF_RING);  // [WARPS][16][DV]
     float* ml = reinterpret_cast<float*>(smem);                  // [WARPS][16][2]: over Q
-    static_assert(WARPS * 16 * DV * 4 <= WARPS * STAGES * Cfg::STAGE && WARPS * 16 * 8 <= 16 * HD * 2, "few rows: shared memory of the join");
+    static_assert(WARPS * 16 * DV * 4 <= WARPS * Cfg::RING && WARPS * 16 * 8 <= 16 * HD * 2, "few rows: shared memory of the join");
     {
         const int r = lane >> 2;
         if ((lane & 3) == 0)
