@@ -80,6 +80,11 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
     const int all_first = k_lo / 16, all_last = k_hi > k_lo ? (k_hi + 15) / 16 : all_first;
     const int first = min(all_last, all_first + split * p.part), last = min(all_last, first + p.part);
     const int words = (last - first + 31) / 32;
+    if (p.nsplit > 1 && first == last) {  // a short sequence's later parts: their slot on the SM is wanted
+        if (half == 0 && (int)threadIdx.x < rows)
+            p.part_lse[((long)split * p.q_rows + sq.q0 + threadIdx.x / p.G) * p.nh + g * p.G + threadIdx.x % p.G] = -INFINITY;
+        return;
+    }
 
     if (p.q_doc)
         for (int w = threadIdx.x; w < words; w += blockDim.x) blocks[w] = 0u;
