@@ -89,13 +89,15 @@ EG2_DEV float4 ams_load4(const T* p, int n, bool vec) {  // n valid elements
 }
 
 template <typename T, int NCH, int RPT>
-__global__ void __launch_bounds__(256) attention_masked_simt_kernel(const MaskedParams p, int q_tiles, int vec) {
+__global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_masked_simt_kernel(const MaskedParams p, int q_tiles, int vec) {
     constexpr int TR = 16 * RPT, QLD = 64 * NCH + 4;
     extern __shared__ float ams_smem[];
     float* qs = ams_smem;                 // [TR][QLD]
     float* kv = qs + TR * QLD;            // [64][AMS_LD]
     float* ps = kv + 64 * AMS_LD;         // [TR][AMS_LD]
     int* docs = (int*)(ps + TR * AMS_LD); // [64]
+    uint32_t* marked = (uint32_t*)(docs + 64);  // [part]: with documents, the key tiles that hold a key of some row's
+    __shared__ int doc_range[2];
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     // Heavy tiles first: under a causal mask the last queries see the most keys.
     long id = blockIdx.x;
@@ -131,19 +133,32 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
     }
     // The union of the rows' ranges, and the documents that they belong to.
     const int t_first = r0 / p.G, t_last = (min(n_rows, r0 + TR) - 1) / p.G;
-    int k_lo, k_hi, tmp, doc_lo = 0, doc_hi = 0;
+    int k_lo, k_hi, tmp;
     masked_range(p, sq, sq.nk - sq.nq + t_first, k_lo, tmp);
     masked_range(p, sq, sq.nk - sq.nq + t_last, tmp, k_hi);
-    if (p.q_doc) {
-        doc_lo = doc_hi = p.q_doc[sq.q0 + t_first];
-        for (int t = t_first + 1; t <= t_last; t++) {
-            const int d = p.q_doc[sq.q0 + t];
-            doc_lo = min(doc_lo, d);
-            doc_hi = max(doc_hi, d);
-        }
-    }
     const int first = k_lo / 64, tiles = k_hi > k_lo ? (k_hi + 63) / 64 - first : 0;
     const int j_first = first + min(tiles, split * p.part), j_last = min(first + tiles, j_first + p.part);
+    if (p.q_doc) {
+        if (tid < 2) doc_range[tid] = tid ? INT_MIN : INT_MAX;
+        for (int x = tid; x < (j_last - j_first + 31) / 32; x += 256) marked[x] = 0u;
+        __syncthreads();
+        if (tid <= t_last - t_first) {
+            const int d = p.q_doc[sq.q0 + t_first + tid];
+            atomicMin(&doc_range[0], d);
+            atomicMax(&doc_range[1], d);
+        }
+        __syncthreads();
+        const int doc_lo = doc_range[0], doc_hi = doc_range[1];
+        for (int x = tid; x < (j_last - j_first) * 64; x += 256) {
+            const int key = j_first * 64 + x;
+            if (key < sq.nk) {
+                const int d = p.k_doc[sq.k0 + key];
+                if (d >= doc_lo && d <= doc_hi) atomicOr(&marked[x >> 11], 1u << ((x >> 6) & 31));
+            }
+        }
+        __syncthreads();
+    }
+
 
     float m[RPT], l[RPT], o[NCH][RPT][4];
 #pragma unroll
@@ -172,16 +187,9 @@ __global__ void __launch_bounds__(256) attention_masked_simt_kernel(const Masked
 #pragma unroll
             for (int x = 0; x < 4; x++) *reinterpret_cast<float4*>(kv + (lr + 16 * x) * AMS_LD + lc) = st[x];
         };
+        if (p.k_doc && !((marked[(j - j_first) >> 5] >> ((j - j_first) & 31)) & 1u)) continue;
         __syncthreads();  // the previous tile's V and documents are done with
-        if (p.k_doc) {
-            bool hit = false;
-            if (tid < 64 && key0 + tid < sq.nk) {
-                const int d = p.k_doc[sq.k0 + key0 + tid];
-                docs[tid] = d;
-                hit = d >= doc_lo && d <= doc_hi;
-            }
-            if (!__syncthreads_or(hit)) continue;
-        }
+        if (p.k_doc && tid < 64) docs[tid] = key0 + tid < sq.nk ? p.k_doc[sq.k0 + key0 + tid] : 0;
         fetch(K, p.ldk, 0);
         float s[RPT][4];
 #pragma unroll
@@ -395,28 +403,34 @@ __global__ void __launch_bounds__(256) attention_masked_join_kernel(const Masked
 template <typename T, int NCH, int RPT>
 static int launch_masked_simt(const MaskedParams& p, int vec, cudaStream_t s) {
     constexpr int TR = 16 * RPT;
-    constexpr int SMEM = (TR * (64 * NCH + 4) + 64 * AMS_LD + TR * AMS_LD + 64) * 4;
+    constexpr int FIXED = (TR * (64 * NCH + 4) + 64 * AMS_LD + TR * AMS_LD + 64) * 4;
+    const int smem = FIXED + (p.q_doc ? (p.part + 31) / 32 * 4 : 0);
     static bool attr_set[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
     auto kern = attention_masked_simt_kernel<T, NCH, RPT>;
     if (!attr_set[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -3;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FIXED + EG2_MASKED_MAX_LEN / 64 / 8) != cudaSuccess) return -3;
         attr_set[dev] = true;
     }
     const int q_tiles = (int)(((long)p.max_q * p.G + TR - 1) / TR);
     const long blocks = (long)q_tiles * p.n_seq * p.nkv;
     if (blocks > 0x7fffffffL) return -1;
-    kern<<<dim3((unsigned)blocks, (unsigned)p.nsplit), 256, SMEM, s>>>(p, q_tiles, vec);
+    kern<<<dim3((unsigned)blocks, (unsigned)p.nsplit), 256, smem, s>>>(p, q_tiles, vec);
     return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-template <typename T>
+template <typename T, int RPT>
 static int attention_masked_simt(const MaskedParams& p, int vec, cudaStream_t s) {
-    if (p.hd <= 64) return launch_masked_simt<T, 1, 4>(p, vec, s);
-    if (p.hd <= 128) return launch_masked_simt<T, 2, 4>(p, vec, s);
-    if (p.hd <= 256) return launch_masked_simt<T, 4, 4>(p, vec, s);
-    return launch_masked_simt<T, 8, 4>(p, vec, s);
+    if (p.hd <= 64) return launch_masked_simt<T, 1, RPT>(p, vec, s);
+    if (p.hd <= 128) return launch_masked_simt<T, 2, RPT>(p, vec, s);
+    if (p.hd <= 256) return launch_masked_simt<T, 4, RPT>(p, vec, s);
+    return launch_masked_simt<T, 8, RPT>(p, vec, s);
+}
+// Rows of a query tile on the CUDA cores: 64 use shared memory best, 32 fill the SMs of a call with few tiles.
+static int masked_simt_rows(const eg2_masked_attention* a) {
+    const long tiles = ((long)a->max_q * (a->nh / a->nkv) + 63) / 64 * a->n_seq * a->nkv;
+    return tiles >= 4L * num_sms() ? 64 : 32;
 }
 
 template <typename T>
@@ -459,7 +473,7 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     // the parts of all sequences are resident at once: their count is at most the key tiles there are (k_rows) over the part,
     // and one more per sequence and head. A part pays for its partial result, 128 rows of it more than one: at least 8 tiles,
     // or 2 where a query tile is mostly empty, or 256 keys in the form for few rows.
-    const int rows = r.few ? 16 : r.tc ? 128 : 64, keys = r.few ? 16 : r.tc ? 128 : 64;
+    const int rows = r.few ? 16 : r.tc ? 128 : masked_simt_rows(a), keys = r.few ? 16 : r.tc ? 128 : 64;
     const int halves = r.tc && a->hd > 256 ? 2 : 1;
     const long tile_rows = (long)a->max_q * r.Gt;
     const long base = (tile_rows + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * halves;
@@ -528,7 +542,10 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
     } else {
         const int unit = a->kind == EG2_F32 ? 16 : 8;  // bytes of four elements
         const int vec = ((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % unit == 0 && (a->ldq | a->ldk | a->ldv | a->hd) % 4 == 0;
-        rc = a->kind == EG2_F32 ? attention_masked_simt<float>(p, vec, s) : attention_masked_simt<bf16_t>(p, vec, s);
+        if (masked_simt_rows(a) == 64)
+            rc = a->kind == EG2_F32 ? attention_masked_simt<float, 4>(p, vec, s) : attention_masked_simt<bf16_t, 4>(p, vec, s);
+        else
+            rc = a->kind == EG2_F32 ? attention_masked_simt<float, 2>(p, vec, s) : attention_masked_simt<bf16_t, 2>(p, vec, s);
     }
     if (!rc && p.nsplit > 1) rc = a->kind == EG2_F32 ? attention_masked_join<float>(p, s) : attention_masked_join<bf16_t>(p, s);
     if (rc == -1) return EG2_ERR_INVALID;

@@ -81,10 +81,10 @@ struct AmtCfg {
     static constexpr int OFF_R = QBUF * QCH * 16384;
     static constexpr int OFF_V = OFF_R + RING * UNIT;
     static constexpr int OFF_UNIT = OFF_V + RING * UNIT;
-    static constexpr int OFF_X = OFF_UNIT + 2 * (int)sizeof(AmtUnit);       // running maxima [2][128]; (maximum, sum) [2][2 groups][128]
-    static constexpr int OFF_TAB = OFF_X + 1024 + 4096;
+    static constexpr int OFF_X = OFF_UNIT + 2 * (int)sizeof(AmtUnit);  // running maxima [2 groups][128]; (maximum, sum) [2][2 groups][128]
+    static constexpr int OFF_TAB = OFF_X + 2048 + 4096;
     static constexpr int OFF_BAR = OFF_TAB + AMT_TABLE * 4;
-    static constexpr int N_BARS = 4 + 2 * QBUF + 4 * RING + 3 * NS + 1 + 8 + 4 + 2 + 2;
+    static constexpr int N_BARS = 4 + 2 * QBUF + 4 * RING + 3 * NS + 1 + 4 + 2 + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + N_BARS * 8 + 16;
 };
 static_assert(AmtCfg<64>::SMEM <= 227 * 1024 && AmtCfg<128>::SMEM <= 227 * 1024 && AmtCfg<256>::SMEM <= 227 * 1024 &&
@@ -287,8 +287,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     uint64_t* p_full = s_full + NS;
     uint64_t* pv_done = p_full + NS;
     uint64_t* o_empty = pv_done + NS;
-    uint64_t* m_bar = o_empty + 1;  // [4 lane quadrants][2]: a row's maximum after a tile (by tile parity)
-    uint64_t* e_bar = m_bar + 8;    // [4]: the groups' maxima and sums of a unit
+    uint64_t* e_bar = o_empty + 1;  // [4 lane quadrants]: the groups' maxima and sums of a unit
     uint64_t* t_bar = e_bar + 4;    // [2]: the bias table may be rewritten; is written
     uint64_t* drain = t_bar + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
@@ -308,7 +307,6 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             mbar_init(&pv_done[x], 1);
         }
         mbar_init(o_empty, 8);
-        for (int x = 0; x < 8; x++) mbar_init(&m_bar[x], 1);
         for (int x = 0; x < 4; x++) mbar_init(&e_bar[x], 2);
         for (int x = 0; x < QBUF; x++) {
             mbar_init(&q_full[x], 1);
@@ -327,6 +325,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         tma_prefetch_desc(&tmV);
     }
     if (warp == 1) tmem_alloc(tmem_slot, 512);
+    // Running maxima, each with the number of its tile in the upper half: none yet.
+    if (threadIdx.x >= 128) reinterpret_cast<unsigned long long*>(smem + Cfg::OFF_X)[threadIdx.x - 128] = ~0ull;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -724,8 +724,23 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const int r = 32 * e + lane;
         const uint32_t lane_off = (uint32_t)(32 * e) << 16;
         constexpr int NC = 128;
-        float* xm = reinterpret_cast<float*>(smem + Cfg::OFF_X);  // [2][128]
-        float* xe = xm + 256;                                     // [2][2 groups][128][2]
+        volatile unsigned long long* xm = reinterpret_cast<unsigned long long*>(smem + Cfg::OFF_X);  // [2 groups][128]
+        float* xe = reinterpret_cast<float*>(smem + Cfg::OFF_X + 2048);                              // [2][2 groups][128][2]
+        // The row's maximum after the other group's tile `tile`: the same thread of that group writes value and number at once,
+        // and writes its next only after it has read this group's answer.
+        auto maximum_after = [&](int tile, bool& ok) -> float {
+            unsigned long long v = xm[(wg ^ 1) * 128 + r];
+            if ((int)(v >> 32) != tile) {
+                const uint64_t t0 = globaltimer_ns();
+                for (uint32_t it = 1; ok && (int)((v = xm[(wg ^ 1) * 128 + r]) >> 32) != tile; it++)
+                    if ((it & 255u) == 0u && (*abort_flag || *(volatile int*)&eg2_dev_status != 0 || globaltimer_ns() - t0 > EG2_WAIT_LIMIT_NS)) {
+                        if (!*abort_flag) eg2_record_error(EG2_DEV_TIMEOUT_ATTN);
+                        *abort_flag = 1;
+                        ok = false;
+                    }
+            }
+            return __uint_as_float((uint32_t)v);
+        };
         float* table = reinterpret_cast<float*>(smem + Cfg::OFF_TAB);
         const int tab_ld = 2 * p.radius + 1 + 256;  // 128 copies of either end around the table
         // Scores are kept as v with the score (log2 domain) v * sc: the scale is left to the exponent's FMA where nothing
@@ -918,13 +933,11 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     // The row's maximum so far comes from the other group's tile, and goes on to its next.
                     float before = AMT_NONE;
                     if (j >= 1) {
-                        if (ok) ok = mbar_wait(&m_bar[2 * e + (wg ^ 1)], ((tile - 1) >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
-                        before = *(volatile float*)&xm[(wg ^ 1) * 128 + r];
+                        if (ok) before = maximum_after(tile - 1, ok);
+                        ok = __all_sync(0xffffffffu, ok);
                     }
                     const float now = (mt - before > ATT_RESCALE_LOG2 || before == AMT_NONE) ? fmaxf(mt, AMT_NONE) : before;
-                    xm[wg * 128 + r] = now;
-                    __syncwarp();
-                    mbar_arrive_if(&m_bar[2 * e + wg], lane == 0);
+                    xm[wg * 128 + r] = (unsigned long long)(uint32_t)tile << 32 | __float_as_uint(now);
                     l *= ex2_approx(m - now);
                     m = now;
                     if (__any_sync(0xffffffffu, now != before && before != AMT_NONE)) {
