@@ -477,7 +477,8 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     const int halves = r.tc && a->hd > 256 ? 2 : 1;
     const long tile_rows = (long)a->max_q * r.Gt;
     const long base = (tile_rows + rows - 1) / rows * a->n_seq * (a->nh / r.Gt) * halves;
-    const long key_tiles = ((long)a->max_k + keys - 1) / keys;
+    const long longest = a->max_k < a->k_rows ? a->max_k : a->k_rows;
+    const long key_tiles = (longest + keys - 1) / keys;
     const long slots = num_sms() * (r.few && halves == 1 ? 2L : 1L);
     long all = base * key_tiles;
     if (a->n_seq > 0 && base / a->n_seq * ((a->k_rows + keys - 1) / keys + a->n_seq) < all) all = base / a->n_seq * ((a->k_rows + keys - 1) / keys + a->n_seq);

@@ -527,7 +527,8 @@ static int launch_i8(const int8_t* A, long lda, const int8_t* W, long ldw, I8Par
     if (tiles > 0x7fffffffL) return -1;
     // 24 MB of weights per panel: a fifth of L2, which also holds the rows passing by.
     const long per_panel = (24L << 20) / ((long)Cfg::BN * p.K);
-    p.panel = per_panel < 1 ? 1 : per_panel > 4096 ? 4096 : (int)per_panel;
+    const long tiles_n = ((long)p.N + Cfg::BN - 1) / Cfg::BN;
+    p.panel = per_panel < 1 ? 1 : per_panel > tiles_n ? (int)tiles_n : (int)per_panel;
     const int n = tiles < clusters_max[dev] ? (int)tiles : clusters_max[dev];
     cfg.gridDim = dim3((PAIR ? 2 : 1) * n, 1, 1);
     attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -86,8 +86,8 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         "eg2_rotary_steps": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.POINTER(C.c_uint64), _FP]),
         "eg2_rotary": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, C.c_int64, C.c_int, _P, C.c_int64, C.c_int, _P, C.c_int64,
                                  _P, C.c_int64, _P, C.c_int64, C.c_int, C.c_int, _P, C.c_float, _P]),
-        "eg2_attention_masked_workspace": (C.c_int64, [C.POINTER(MaskedAttention)]),
-        "eg2_attention_masked": (C.c_int, [C.POINTER(MaskedAttention), _P, C.c_int64, _P]),
+        "eg2_attention_masked_workspace": (C.c_int64, [_P]),  # a MaskedAttention by reference, or its bytes
+        "eg2_attention_masked": (C.c_int, [_P, _P, C.c_int64, _P]),
         "eg2_quantize_rows": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int, _P]),
         "eg2_gemm_i8": (C.c_int, [_P, C.c_int64, _P, _P, C.c_int64, _P, _P, _P, C.c_int64, C.c_int64, C.c_int, C.c_int,
                                   C.c_int, _P]),

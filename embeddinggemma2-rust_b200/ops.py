@@ -7,18 +7,22 @@ prefix masks, weights held in 8 bits. Each call launches the library's kernels o
 its tensors' device and returns without waiting; results are new tensors unless ``out`` is given. A tensor of
 the wrong type, shape, stride or device, and what the library refuses, raises :class:`lib.Eg2Error`.
 
+A bounded device wait that ran out is not raised by the call: after synchronising, ``eg2_device_status`` tells.
 A tensor that is used on another stream than the one it was made on is kept alive and ordered by the caller,
 as for any torch operation.
 """
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
 
 from . import lib as L
 
+_MASKED = struct.Struct("@iPPPPPqqqqPPqqiiiiiiffiiPPPPPi0P")  # eg2_masked_attention
+assert _MASKED.size == C.sizeof(L.MaskedAttention)
 KINDS = {torch.bfloat16: L.EG2_BF16, torch.float32: L.EG2_F32}
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
@@ -195,19 +199,18 @@ def attention_masked(q, k, v, q_off, k_off, max_q: int, max_k: int, *, scale: fl
     lse = torch.empty(q_rows, nh, dtype=torch.float32, device=q.device) if return_lse else None
 
     def ptr(t):
-        return None if t is None else t.data_ptr()
+        return 0 if t is None else t.data_ptr()
 
-    a = L.MaskedAttention(KINDS[kind], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(lse), ldq, ldk, ldv, ldo,
-                          q_off.data_ptr(), k_off.data_ptr(), q_rows, k_rows, n_seq, int(max_q), int(max_k), nh, nkv, hd,
-                          scale, softcap, int(window), 1 if causal else 0, ptr(prefix_len), ptr(q_doc), ptr(k_doc),
-                          ptr(slopes), ptr(dist_bias), radius)
+    a = _MASKED.pack(KINDS[kind], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(lse), ldq, ldk, ldv, ldo,
+                     q_off.data_ptr(), k_off.data_ptr(), q_rows, k_rows, n_seq, int(max_q), int(max_k), nh, nkv, hd, scale, softcap,
+                     int(window), 1 if causal else 0, ptr(prefix_len), ptr(q_doc), ptr(k_doc), ptr(slopes), ptr(dist_bias), radius)
     lib = L.load()
-    need = lib.eg2_attention_masked_workspace(C.byref(a))
+    need = lib.eg2_attention_masked_workspace(a)
     if need < 0:
         _check(int(need), "attention_masked")
     # From torch's allocator on this stream, so calls on several streams do not share it.
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _check(lib.eg2_attention_masked(C.byref(a), ptr(work), need, stream), "attention_masked")
+    _check(lib.eg2_attention_masked(a, ptr(work), need, stream), "attention_masked")
     return (out, lse) if return_lse else out
 
 

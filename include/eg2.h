@@ -159,7 +159,8 @@ int eg2_attention_noalloc(const void* q, const void* k, const void* v, void* out
 /* ---- operators of one encoder layer in other forms than the two towers use ----------------------
  * No counterpart in the reference. All three take device pointers, allocate nothing, copy nothing, run
  * asynchronously on `stream` (NULL: the default stream) and check what the host can see before they launch
- * (EG2_ERR_INVALID, nothing written). kind: EG2_BF16 or EG2_F32, the type of the activations; arithmetic,
+ * (EG2_ERR_INVALID, nothing written). A bounded device wait that ran out is not returned: synchronise the stream, then
+ * read eg2_device_status() (non-zero: results since then are not valid). kind: EG2_BF16 or EG2_F32, the type of the activations; arithmetic,
  * sums and softmax statistics are f32. Row strides are in elements; the channels of a head and the heads of
  * a row are contiguous. */
 
