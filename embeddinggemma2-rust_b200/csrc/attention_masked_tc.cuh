@@ -63,6 +63,7 @@ struct AmtParams {
 
 template <int HD>
 struct AmtCfg {
+    static constexpr int R_AUX = HD <= 128 ? 56 : 72, R_SOFT = HD <= 128 ? 224 : 216;  // registers (measured: 2 % to 8 % either way)
     static constexpr int QCH = HD / 64;                   // 16 KB chunks of Q
     static constexpr int QBUF = HD <= 128 ? 2 : 1;        // Q buffers: the next unit's Q lands under this one
     static constexpr int UCH = HD == 128 || HD == 256 ? 2 : 1;  // 64-channel chunks per ring unit (128 keys each)
@@ -265,7 +266,14 @@ EG2_DEV void guard_chunk(uint8_t* chunk, int live, bool scrub, AmtUnit& u, int k
     }
 }
 
-template <int HD>
+// The score's parts that a kernel is compiled for; AMT_ANY decides at run time. The softmax is long straight code, and what
+// a call does not need costs it instruction fetches. 8,192 tokens, 8 heads of 64 / 128 / 256, decided at run time and
+// compiled for the call: plain 427 / 323 / 289 and 432 / 279 / 269 us, capped 742 / 523 / 375 and 657 / 474 / 345, slopes
+// 593 / 447 / 338 and 545 / 386 / 300, a table 701 / 546 / 349 and 584 / 411 / 319. `raw` below stays a test at run time in
+// each: with it known, the compiler mixes the parts with the mask's code and spills (table 588 / 560 / 378 us).
+constexpr int AMT_CAP = 1, AMT_SLOPES = 2, AMT_TAB = 4, AMT_ANY = 8;
+
+template <int HD, int PARTS>
 __global__ void __launch_bounds__(AMT_THREADS, 1)
     attention_masked_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AmtParams ap) {
@@ -347,7 +355,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // The block starts with 168 registers a thread: 3 x 168 = R_AUX + 2 R_SOFT.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::R_AUX));
         if (warp == 0 && lane == 0) {
             int k_loads = 0, v_loads = 0, q_loads = 0;
             if constexpr (!Cfg::POLL) {
@@ -719,7 +728,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::R_SOFT));
         const int e = warp & 3, wg = (warp - 4) >> 2;
         const int r = 32 * e + lane;
         const uint32_t lane_off = (uint32_t)(32 * e) << 16;
@@ -745,17 +754,19 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const int tab_ld = 2 * p.radius + 1 + 256;  // 128 copies of either end around the table
         // Scores are kept as v with the score (log2 domain) v * sc: the scale is left to the exponent's FMA where nothing
         // needs it before (sc > 0, so the order is kept).
-        const bool capped = p.softcap > 0.f;
+        const bool capped = PARTS == AMT_ANY ? p.softcap > 0.f : (PARTS & AMT_CAP) != 0;
+        const bool slopes = PARTS == AMT_ANY ? p.slopes != nullptr : (PARTS & AMT_SLOPES) != 0;
+        const bool tables = PARTS == AMT_ANY ? p.table != nullptr : (PARTS & AMT_TAB) != 0;
         const float cap2 = p.softcap * AMT_LOG2E;
         const float a = capped ? p.scale / p.softcap : p.scale * AMT_LOG2E;
-        const bool raw = !capped && !p.slopes && !p.table && a > 0.f;
+        const bool raw = !(p.softcap > 0.f) && !p.slopes && !p.table && a > 0.f;
         const float sc = raw ? a : 1.f;
         // cap2 tanh(a s) = s (c0 + c1 s^2 + ...) where |a s| <= 1/2, as long as the powers of a stay in range.
         const bool near_ok = fabsf(a) > 1e-4f && fabsf(a) < 1e3f;
         const float near_max = near_ok ? (AMT_TANH_MAX / a) * (AMT_TANH_MAX / a) : -1.f;
         const float c0 = AMT_T0 * a * cap2, c1 = AMT_T1 * a * a * a * cap2, c2 = AMT_T2 * (a * a) * (a * a) * a * cap2,
                     c3 = AMT_T3 * (a * a * a) * (a * a * a) * a * cap2, c4 = AMT_T4 * (a * a * a) * (a * a * a) * (a * a * a) * cap2;
-        int T = 0, U = 0, tab_head = -1, tables = 0;
+        int T = 0, U = 0, tab_head = -1, builds = 0;
         bool ok = true;
 
         for (int i = 0; ok; i++) {
@@ -771,21 +782,21 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 masked_range(p, un->sq, place, lo, hi);
                 if (p.q_doc) qdoc = p.q_doc[un->sq.q0 + tok];
             }
-            const float slope = (p.slopes && live) ? p.slopes[head] * AMT_LOG2E : 0.f;
-            if (p.table && un->rows > 0 && tab_head != un->head0) {
+            const float slope = (slopes && live) ? p.slopes[head] * AMT_LOG2E : 0.f;
+            if (tables && un->rows > 0 && tab_head != un->head0) {
                 tab_head = un->head0;
                 const int s_tid = threadIdx.x - 128;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_bar[0]);
-                if (!(ok = mbar_wait(&t_bar[0], tables & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                if (!(ok = mbar_wait(&t_bar[0], builds & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
                 for (int x = s_tid; x < ap.Gt * tab_ld; x += 256) {
                     const int hh = x / tab_ld, c = min(max(x % tab_ld - 128, 0), 2 * p.radius);
                     table[x] = masked_bias(p.table[(long)(tab_head + hh) * (2 * p.radius + 1) + c]) * AMT_LOG2E;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_bar[1]);
-                if (!(ok = mbar_wait(&t_bar[1], tables & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
-                tables++;
+                if (!(ok = mbar_wait(&t_bar[1], builds & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                builds++;
             }
             const float* my_table = table + (r % ap.Gt) * tab_ld;
             float m = AMT_NONE, l = 0.f;  // the row's maximum at this group's last tile, and its part of the sum in units of 2^m
@@ -899,12 +910,12 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
 #pragma unroll
                                 for (int c = 0; c < NC; c += 2) f2_unpack(f2_mul(f2_pack(sv[c], sv[c + 1]), a2), sv[c], sv[c + 1]);
                             }
-                            if (p.slopes) {
+                            if (slopes) {
                                 const float d0 = (float)(kbase - place);
 #pragma unroll
                                 for (int c = 0; c < NC; c++) sv[c] = fmaf(-slope, fabsf(d0 + (float)c), sv[c]);
                             }
-                            if (p.table) {
+                            if (tables) {
                                 // j - i runs over 128 consecutive values: clamped once, the copies of the ends do the rest.
                                 const float* tb = my_table + min(max(kbase - place, -p.radius - 128), p.radius) + p.radius + 128;
 #pragma unroll
@@ -1111,10 +1122,10 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     }
 }
 
-template <int HD>
+template <int HD, int PARTS>
 static int launch_masked_tc(const MaskedParams& p, int Gt, cudaStream_t s) {
     using Cfg = AmtCfg<HD>;
-    auto kern = attention_masked_tc_kernel<HD>;
+    auto kern = attention_masked_tc_kernel<HD, PARTS>;
     static bool attr_set[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
@@ -1148,4 +1159,19 @@ static int launch_masked_tc(const MaskedParams& p, int Gt, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, ap) == cudaSuccess ? 0 : -3;
+}
+
+// The kernel compiled for just this call's score, where there is one (the plain score keeps its scale for the exponent,
+// which wants it positive).
+template <int HD>
+static int launch_masked_tc(const MaskedParams& p, int Gt, cudaStream_t s) {
+    const int parts = (p.softcap > 0.f ? AMT_CAP : 0) | (p.slopes ? AMT_SLOPES : 0) | (p.table ? AMT_TAB : 0);
+    switch (parts) {
+        case 0: return p.scale > 0.f ? launch_masked_tc<HD, 0>(p, Gt, s) : launch_masked_tc<HD, AMT_ANY>(p, Gt, s);
+        case AMT_CAP: return launch_masked_tc<HD, AMT_CAP>(p, Gt, s);
+        case AMT_SLOPES: return launch_masked_tc<HD, AMT_SLOPES>(p, Gt, s);
+        case AMT_TAB: return launch_masked_tc<HD, AMT_TAB>(p, Gt, s);
+        case AMT_CAP | AMT_SLOPES: return launch_masked_tc<HD, AMT_CAP | AMT_SLOPES>(p, Gt, s);
+        default: return launch_masked_tc<HD, AMT_ANY>(p, Gt, s);
+    }
 }
