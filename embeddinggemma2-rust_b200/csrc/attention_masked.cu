@@ -400,6 +400,44 @@ __global__ void __launch_bounds__(256) attention_masked_join_kernel(const Masked
     }
 }
 
+// The same for up to JOIN_PARTS parts, a warp per row: many rows with few parts each are bound by reading the parts, and a
+// block per row is mostly waiting (call of 1,000 queries, 4 heads over 2 of 256, 8,192 keys in 4 parts: 59 us with it, 83 with
+// a block per row; of 32 queries in 8 parts: 38 and 34).
+constexpr int JOIN_PARTS = 8;
+template <typename T>
+__global__ void __launch_bounds__(256) attention_masked_join_rows_kernel(const MaskedParams p) {
+    grid_dep_launch();
+    grid_dep_wait();
+    const int lane = threadIdx.x & 31;
+    long id = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (id >= (long)p.n_seq * p.max_q * p.nh) return;
+    const int h = (int)(id % p.nh);
+    id /= p.nh;
+    const int t = (int)(id % p.max_q), b = (int)(id / p.max_q);
+    const MaskedSeq sq = masked_seq(p, b);
+    if (t >= sq.nq) return;
+    const long row = sq.q0 + t, item = row * p.nh + h, step = p.q_rows * p.nh;
+    const float lse = lane < p.nsplit ? p.part_lse[lane * step + item] : -INFINITY;
+    float top = lse;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top, mine = expf(lse - base);
+    float w[JOIN_PARTS], total = 0.f;
+#pragma unroll
+    for (int s = 0; s < JOIN_PARTS; s++) total += w[s] = __shfl_sync(0xffffffffu, mine, s);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll 4
+    for (int c = lane; c < p.hd; c += 32) {
+        float o[JOIN_PARTS], sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < JOIN_PARTS; s++) o[s] = w[s] != 0.f ? p.part_o[(s * step + item) * p.hd + c] : 0.f;
+#pragma unroll
+        for (int s = 0; s < JOIN_PARTS; s++) sum = fmaf(w[s], o[s], sum);
+        stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, sum * inv);
+    }
+    if (lane == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+}
+
 template <typename T, int NCH, int RPT>
 static int launch_masked_simt(const MaskedParams& p, int vec, cudaStream_t s) {
     constexpr int TR = 16 * RPT;
@@ -427,15 +465,19 @@ static int attention_masked_simt(const MaskedParams& p, int vec, cudaStream_t s)
     if (p.hd <= 256) return launch_masked_simt<T, 4, RPT>(p, vec, s);
     return launch_masked_simt<T, 8, RPT>(p, vec, s);
 }
-// Rows of a query tile on the CUDA cores: 64 use shared memory best, 32 fill the SMs of a call with few tiles.
+// Rows of a query tile on the CUDA cores: 64 use shared memory best, 32 fill the SMs of a call with few tiles (f32, 64 / 32
+// rows: 256 tiles of 64, 4,096 tokens, 4 heads over 1 of 128: 1,471 / 1,732 us; 192 tiles, 1,000 tokens, 12 heads of 64:
+// 226 / 196; 32 tiles, 500 tokens, 4 heads over 2 of 256: 174 / 132).
 static int masked_simt_rows(const eg2_masked_attention* a) {
     const long tiles = ((long)a->max_q * (a->nh / a->nkv) + 63) / 64 * a->n_seq * a->nkv;
-    return tiles >= 4L * num_sms() ? 64 : 32;
+    return tiles >= num_sms() * 3L / 2 ? 64 : 32;
 }
 
 template <typename T>
 static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
-    const long blocks = (long)p.n_seq * p.max_q * p.nh;
+    const long items = (long)p.n_seq * p.max_q * p.nh;
+    const bool by_rows = p.nsplit <= JOIN_PARTS && items > 4L * num_sms();
+    const long blocks = by_rows ? (items + 7) / 8 : items;
     if (blocks > 0x7fffffffL) return -1;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -443,18 +485,20 @@ static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)blocks, 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
-    cfg.dynamicSmemBytes = (p.nsplit + p.hd) * 4;
+    cfg.dynamicSmemBytes = by_rows ? 0 : (p.nsplit + p.hd) * 4;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, attention_masked_join_kernel<T>, p) == cudaSuccess ? 0 : -3;
+    return cudaLaunchKernelEx(&cfg, by_rows ? attention_masked_join_rows_kernel<T> : attention_masked_join_kernel<T>, p) == cudaSuccess ? 0 : -3;
 }
 
 // How a call runs. The tensor cores take bf16 whose rows and heads TMA can address (16-byte multiples) and G query
 // heads that divide a 128-row tile are packed into it, unless their bias tables together pass the shared memory
 // kept for them; the rest runs on the CUDA cores. Calls whose query tiles would be at most an eighth full -- 16 rows --
-// are bound by reading K and V and take the form made for that (8 queries, 4 heads over 2 of 256, up to 11,774 keys: 75 us in
-// 128-row tiles).
+// are bound by reading K and V and take the form made for that (4 heads over 2 of 256, up to 8 x 11,774 keys: 1 query each 43 us,
+// 60 in 128-row tiles, 8 queries each 55 and 63; 64 x 512 keys, 12 heads of 64: 47 and 71; only at a few hundred keys and all 16
+// rows do the tiles win: 8 queries over 300, 22 and 19). Packing: 256 sequences of 17 tokens, 4 heads over 1 of 256, 24 us, 64
+// with a tile per head.
 struct MaskedPlan {
     bool tc, few;
     int Gt, nsplit, part;
@@ -472,7 +516,10 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     // The key axis is split into parts of a fixed number of key tiles when the query tiles alone leave SMs idle, so many that
     // the parts of all sequences are resident at once: their count is at most the key tiles there are (k_rows) over the part,
     // and one more per sequence and head. A part pays for its partial result, 128 rows of it more than one: at least 8 tiles,
-    // or 2 where a query tile is mostly empty, or 256 keys in the form for few rows.
+    // or 2 where a query tile is mostly empty (each with as much again to share), or a block of 16 keys for each warp of the form
+    // for few rows (two at head 512). Split and whole: 2,000 queries, 4 heads over 2 of 256, 8,192 keys 90 / 129 us; 256 queries,
+    // 12 heads of 64, 2,048 keys 21 / 22; 1,200 over as many in two parts of 5 tiles 35 / 29 (hence the 8); 1 query over 2,208
+    // keys 14 / 55.
     const int rows = r.few ? 16 : r.tc ? 128 : masked_simt_rows(a), keys = r.few ? 16 : r.tc ? 128 : 64;
     const int halves = r.tc && a->hd > 256 ? 2 : 1;
     const long tile_rows = (long)a->max_q * r.Gt;
@@ -483,9 +530,10 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     long all = base * key_tiles;
     if (a->n_seq > 0 && base / a->n_seq * ((a->k_rows + keys - 1) / keys + a->n_seq) < all) all = base / a->n_seq * ((a->k_rows + keys - 1) / keys + a->n_seq);
     long part = base < slots ? (all + slots - base - 1) / (slots - base) : key_tiles;
-    const long least = r.few ? 16 : tile_rows > rows / 4 ? 8 : 2;
+    const long least = r.few ? (a->hd > 256 ? 8 : 4) : tile_rows > rows / 4 ? 8 : 2;
     if (part < least) part = least;
-    r.nsplit = base >= slots || part >= key_tiles ? 1 : (int)((key_tiles + part - 1) / part);
+    r.nsplit = base >= slots || part >= key_tiles || (!r.few && key_tiles < 2 * least) ? 1 : (int)((key_tiles + part - 1) / part);
+    if (r.nsplit > 1 && base * r.nsplit <= slots) part = (key_tiles + r.nsplit - 1) / r.nsplit;
     r.part = r.nsplit > 1 ? (int)part : (int)(key_tiles > 0 ? key_tiles : 1);
     return r;
 }

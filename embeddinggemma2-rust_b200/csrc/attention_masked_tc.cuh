@@ -267,8 +267,8 @@ EG2_DEV void guard_chunk(uint8_t* chunk, int live, bool scrub, AmtUnit& u, int k
 }
 
 // The score's parts that a kernel is compiled for; AMT_ANY decides at run time. The softmax is long straight code, and what
-// a call does not need costs it instruction fetches. 8,192 tokens, 8 heads of 64 / 128 / 256, decided at run time and
-// compiled for the call: plain 427 / 323 / 289 and 432 / 279 / 269 us, capped 742 / 523 / 375 and 657 / 474 / 345, slopes
+// a call does not need costs it instruction fetches. 8,192 tokens, 12 heads of 64 / 8 over 2 of 128 / 4 over 2
+// of 256, decided at run time and compiled for the call: plain 427 / 323 / 289 and 432 / 279 / 269 us, capped 742 / 523 / 375 and 657 / 474 / 345, slopes
 // 593 / 447 / 338 and 545 / 386 / 300, a table 701 / 546 / 349 and 584 / 411 / 319. `raw` below stays a test at run time in
 // each: with it known, the compiler mixes the parts with the mask's code and spills (table 588 / 560 / 378 us).
 constexpr int AMT_CAP = 1, AMT_SLOPES = 2, AMT_TAB = 4, AMT_ANY = 8;

