@@ -281,6 +281,19 @@ def test_attention_few_queries_over_many_keys(dtype, nh, nkv, hd, nq, causal):
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("nq", [100, 330])
+@pytest.mark.parametrize("docs", [False, True])
+def test_attention_split_over_many_rows(dtype, nh, nkv, hd, nq, docs):
+    """Hundreds of queries over a split key axis: parts without a key of a row's, rows without any key."""
+    ql, kl, q_doc, k_doc = [nq, 0, 5], [4000, 3, 40], None, None
+    if docs:
+        k_doc = (torch.arange(sum(kl), dtype=torch.int32) // 600).cuda()
+        q_doc = (torch.arange(sum(ql), dtype=torch.int32) % 9).cuda()
+    run_case(dtype, nh, nkv, hd, ql, kl, softcap=20.0, q_doc=q_doc, k_doc=k_doc)
+    run_case(dtype, nh, nkv, hd, ql, kl, causal=True, window=900, q_doc=q_doc, k_doc=k_doc)
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 @pytest.mark.parametrize("few", [False, True])
 def test_hidden_keys_may_hold_anything(dtype, nh, nkv, hd, few):
     """NaN and infinities in keys and values that the masks hide -- rows between sequences, other documents, keys
