@@ -50,7 +50,8 @@ EG2_DEV void masked_range(const MaskedParams& p, const MaskedSeq& s, int i, int&
     lo = 0;
     hi = s.nk;
     if (p.window >= 0) {
-        lo = max(0, i - p.window);
+        // In 64 bits on both sides: places of queries beyond the keys are negative, windows any int.
+        lo = (int)max(0l, (long)i - p.window);
         hi = min(hi, (int)min((long)i + p.window + 1, (long)s.nk));
     }
     if (p.causal) hi = min(hi, max(i + 1, s.prefix));
