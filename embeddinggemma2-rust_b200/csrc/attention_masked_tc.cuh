@@ -868,7 +868,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         if (!raw) {
                             if (capped) {
                                 // The polynomial for every score, four pairs at a time; where one is out of its range the
-                                // tile is done again from S, 16 columns at a time through TMEM.
+                                // tile is done again from S, 16 columns at a time through TMEM. Each score keeps the form that its
+                                // own size asks for, so its bits do not depend on its neighbours, hidden ones among them.
                                 float far = 0.f;
 #pragma unroll
                                 for (int c = 0; c < NC; c += 8) {
@@ -902,7 +903,11 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                                         tmem_ld_wait();
                                         reg_fence<16>(o);
 #pragma unroll
-                                        for (int q = 0; q < 16; q++) o[q] = __float_as_uint(cap2 * tanh_any(__uint_as_float(o[q]) * a));
+                                        for (int q = 0; q < 16; q++) {
+                                            const float x = __uint_as_float(o[q]), y = x * x;
+                                            const float near = x * fmaf(fmaf(fmaf(fmaf(y, c4, c3), y, c2), y, c1), y, c0);
+                                            o[q] = __float_as_uint(y <= near_max ? near : cap2 * tanh_any(x * a));
+                                        }
                                         tmem_st16(ts + c, o);
                                     }
                                     tmem_st_wait();
