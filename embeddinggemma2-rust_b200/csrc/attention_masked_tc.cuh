@@ -30,15 +30,16 @@
 //
 // Hidden keys are masked by selection, so what K holds there is harmless, but a NaN or infinity in a hidden V row
 // would reach the sum as 0 x NaN. Rows past the sequence's end are zeroed in shared memory by the P V warp. Other
-// hidden rows are taken to be finite; a unit with masked tiles whose result is not finite is run once more with
-// every V tile cleaned there (non-finite elements to 0, their keys listed), and a row that sees a listed
-// key is then computed again from its visible keys alone (masked_row_again). So no visible bit depends on what
-// hidden keys hold, at no cost while all is finite.
+// hidden rows are taken to be finite; a unit with masked tiles whose result is not finite is run again in stages
+// (AmtUnit::stage): once with the elements of V that are not finite set to 0, which gives every row its finite sum, then
+// twice over the tiles that held such elements, with 1 for each of them in V and 1 for each visible key in P: where this
+// product is positive the row sees an infinity of that sign, or a NaN, in that channel, and takes it. So no visible bit
+// depends on what hidden keys hold, at no cost while all is finite; where it is not, a unit's time grows by its one
+// repetition and the tiles concerned, whatever their number, never by rows taken one by one.
 
 constexpr int AMT_THREADS = 384;
 constexpr int AMT_MASK_WORDS = EG2_MASKED_MAX_LEN / 128 / 32;
 constexpr int AMT_TABLE = 4096;  // floats of distance bias in shared memory
-constexpr int AMT_BAD = 64;
 constexpr float AMT_LOG2E = 1.4426950408889634f;
 constexpr float AMT_NONE = -3e38f;  // the maximum of a row that has seen nothing
 
@@ -49,11 +50,14 @@ struct alignas(16) AmtUnit {
     int split, half;  // part of the key axis; 256-channel half of O
     int n, first;     // key tiles to visit; the first (without documents they are consecutive,
     int down;         // and the first `down` of them are visited backwards)
-    int stop, scrub, retry;  // no further unit; clean every V tile; (set by the softmax) run again with scrub
+    int sparse;       // the tiles are those of `visit`
+    int stop;         // no further unit
+    int stage;        // 0 as it is; 1 elements of V that are not finite count as 0; 2, 3 as 1 if +infinity (2), -infinity (3)
+                      // or NaN, else 0, under weights of 1
+    int retry;        // (set by the softmax in stage 0) run again
     int masked;       // (set by the softmax) some tile was masked
-    int n_bad;       // scrub: keys whose V row was not finite (past AMT_BAD of them, any may be)
-    int bad[64];
-    uint32_t visit[AMT_MASK_WORDS], docs[AMT_MASK_WORDS];
+    int found;        // (set by the P V warp in stage 1) some element was not finite: in the tiles of `bad`
+    uint32_t visit[AMT_MASK_WORDS], docs[AMT_MASK_WORDS], bad[AMT_MASK_WORDS];
 };
 
 struct AmtParams {
@@ -144,12 +148,12 @@ EG2_DEV float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// tanh anywhere: past 0.5 as 1 - 2 / (1 + e^2x), good to 2^-21 there (1 where e^2x overflows).
+// tanh past 0.5 as 1 - 2 / (1 + e^2x), good to 2^-21 there (1 where e^2x overflows); anywhere.
+EG2_DEV float tanh_far(float x) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(2.f * AMT_LOG2E * x)); }
 EG2_DEV float tanh_any(float x) {
     const float y = x * x;
     const float near = x * fmaf(fmaf(fmaf(fmaf(AMT_T4, y, AMT_T3), y, AMT_T2), y, AMT_T1), y, AMT_T0);
-    const float far = 1.f - __fdividef(2.f, 1.f + ex2_approx(2.f * AMT_LOG2E * x));
-    return fabsf(x) <= AMT_TANH_MAX ? near : far;
+    return fabsf(x) <= AMT_TANH_MAX ? near : tanh_far(x);
 }
 
 // The set bits of a mask, in order.
@@ -172,101 +176,120 @@ struct TileWalk {
     bool sparse;
     int first, down, j;
     EG2_DEV TileWalk() : bits(nullptr), sparse(false), first(0), down(0), j(0) {}
-    EG2_DEV TileWalk(const AmtUnit& u, bool docs) : bits(u.visit), sparse(docs), first(u.first), down(u.down), j(0) {}
+    EG2_DEV explicit TileWalk(const AmtUnit& u) : bits(u.visit), sparse(u.sparse != 0), first(u.first), down(u.down), j(0) {}
     EG2_DEV int next() {
         const int i = j++;
         return sparse ? bits.next() : first + (i < down ? down - 1 - i : i);
     }
 };
 
-EG2_DEV float masked_score2(const MaskedParams& p, float dot, int head, int apart) {  // in the log2 domain
-    float y = p.softcap > 0.f ? p.softcap * AMT_LOG2E * tanh_any(dot * (p.scale / p.softcap)) : dot * p.scale * AMT_LOG2E;
-    if (p.slopes) y -= p.slopes[head] * AMT_LOG2E * fabsf((float)apart);
-    if (p.table) y += masked_bias(p.table[(long)head * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]) * AMT_LOG2E;
-    return y;
-}
-
-// Channels [c_lo, c_hi) of one row of a unit, from its visible keys only; the whole warp works on it.
-template <int HD>
-__device__ __noinline__ void masked_row_again(const MaskedParams& p, const AmtUnit& u, int r, int Gt, int c_lo, int c_hi) {
-    constexpr int NV = HD / 32;
+// Prepares one 16 KB chunk of a V tile (128 keys of 128 bytes, whatever the order of the 16-byte units in a row) for the
+// unit's stage; rows from `live` on become zero. Whether some other element was not finite.
+EG2_DEV bool guard_chunk(uint8_t* chunk, int live, int stage) {
     const int lane = threadIdx.x & 31;
-    const int t = u.t0 + r / Gt, head = u.head0 + r % Gt;
-    const long row = u.sq.q0 + t;
-    const int place = u.sq.nk - u.sq.nq + t;
-    int lo, hi;
-    masked_range(p, u.sq, place, lo, hi);
-    const int qdoc = p.q_doc ? p.q_doc[row] : 0;
-    const bf16_t* q = (const bf16_t*)p.q + row * p.ldq + (long)head * p.hd;
-    float qv[NV], acc[NV], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int x = 0; x < NV; x++) {
-        qv[x] = lane + 32 * x < p.hd ? ldf(q, lane + 32 * x) : 0.f;
-        acc[x] = 0.f;
-    }
-    TileWalk walk(u, p.q_doc != nullptr);
-    for (int i = 0; i < u.n; i++) {
-        const int kt = walk.next();
-        for (int key = max(lo, kt * 128); key < min(hi, kt * 128 + 128); key++) {
-            const long kr = u.sq.k0 + key;
-            if (p.k_doc && p.k_doc[kr] != qdoc) continue;
-            const bf16_t* kk = (const bf16_t*)p.k + kr * p.ldk + (long)u.g * p.hd;
-            const bf16_t* vv = (const bf16_t*)p.v + kr * p.ldv + (long)u.g * p.hd;
-            float s = 0.f;
-#pragma unroll
-            for (int x = 0; x < NV; x++)
-                if (lane + 32 * x < p.hd) s = fmaf(qv[x], ldf(kk, lane + 32 * x), s);
-            s = masked_score2(p, warp_sum(s), head, key - place);
-            const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-            const float corr = ex2_approx(m - base), w = ex2_approx(s - base);
-            l = l * corr + w;
-            m = mn;
-#pragma unroll
-            for (int x = 0; x < NV; x++) {
-                acc[x] *= corr;
-                if (w != 0.f && lane + 32 * x < p.hd) acc[x] = fmaf(w, ldf(vv, lane + 32 * x), acc[x]);
-            }
-        }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const long at = row * p.nh + head + (p.nsplit > 1 ? (long)u.split * p.q_rows * p.nh : 0);
-#pragma unroll
-    for (int x = 0; x < NV; x++) {
-        const int c = lane + 32 * x;
-        if (c >= c_lo && c < c_hi && c < p.hd) {
-            if (p.nsplit > 1)
-                p.part_o[at * p.hd + c] = acc[x] * inv;
-            else
-                stf((bf16_t*)p.out + row * p.ldo + (long)head * p.hd, c, acc[x] * inv);
-        }
-    }
-}
-
-// Cleans one 16 KB chunk of a V tile (128 keys of 128 bytes, whatever the order of the 16-byte units in a row):
-// rows from `live` on become zero; with `scrub` non-finite elements of the others do, and their keys are listed.
-EG2_DEV void guard_chunk(uint8_t* chunk, int live, bool scrub, AmtUnit& u, int key0) {
-    const int lane = threadIdx.x & 31;
+    bool hit = false;
     for (int x = lane; x < 1024; x += 32) {
-        const int row = x >> 3;
         uint4* at = reinterpret_cast<uint4*>(chunk) + x;
-        if (row >= live) {
+        if ((x >> 3) >= live) {
             *at = make_uint4(0u, 0u, 0u, 0u);
-        } else if (scrub) {
-            uint4 v = *at;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-            bool hit = false;
+        } else if (stage) {
+            const uint4 v = *at;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int y = 0; y < 4; y++) {
-                if ((w[y] & 0x7f80u) == 0x7f80u) w[y] &= 0xffff0000u, hit = true;
-                if ((w[y] & 0x7f800000u) == 0x7f800000u) w[y] &= 0xffffu, hit = true;
+                uint32_t r = 0u;
+#pragma unroll
+                for (int z = 0; z < 32; z += 16) {
+                    const uint32_t e = (w[y] >> z) & 0xffffu;
+                    const bool odd = (e & 0x7f80u) == 0x7f80u, takes = e != (stage == 2 ? 0xff80u : 0x7f80u);  // NaN, or the sign asked for
+                    hit |= odd;
+                    r |= (stage == 1 ? (odd ? 0u : e) : odd && takes ? 0x3f80u : 0u) << z;
+                }
+                w[y] = r;
             }
-            if (hit) {
-                *at = v;
-                const int n = atomicAdd(&u.n_bad, 1);  // a key may be listed more than once
-                if (n < AMT_BAD) u.bad[n] = key0 + row;
-            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
+    return hit;
+}
+
+// A softmax warp's part of a unit in stages 2 and 3: weights of 1 for the visible keys of its group's tiles, then, where the
+// product is positive, the infinity to the sums that stage 1 wrote (of both signs, or with a NaN, they make NaN). False where a
+// wait ran out. Apart from the loop over scores, whose speed goes by what else is compiled into it (8,192 tokens without a mask, 8 heads
+// over 2 of 128: 288 us, 372 with these weights as a branch inside that loop).
+template <int HD>
+EG2_DEV bool masked_count_unit(const AmtParams& ap, const AmtUnit& u, uint32_t tmem, int T, int U, uint64_t* s_full, uint64_t* p_full,
+                               uint64_t* pv_done, uint64_t* o_empty, uint64_t* e_bar, volatile int* abort_flag) {
+    using Cfg = AmtCfg<HD>;
+    constexpr int NS = Cfg::NS;
+    const MaskedParams& p = ap.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = warp & 3, wg = (warp - 4) >> 2, r = 32 * e + lane;
+    const uint32_t mine = tmem + ((uint32_t)(32 * e) << 16);
+    const bool live = r < u.rows;
+    const int t = u.t0 + r / ap.Gt, head = u.head0 + r % ap.Gt;
+    const long row = u.sq.q0 + t;
+    int lo = 0, hi = 0;
+    if (live) masked_range(p, u.sq, u.sq.nk - u.sq.nq + t, lo, hi);
+    const int qdoc = live && p.q_doc ? p.q_doc[row] : 0;
+    TileWalk walk(u);
+    bool ok = true;
+    for (int j = 0; j < u.n; j++) {
+        const int kbase = walk.next() * 128, buf = (T + j) % NS;
+        if (((T + j) & 1) != wg) continue;
+        ok = mbar_wait(&s_full[buf], ((T + j) / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        tc_fence_after();
+        const bool docs = p.q_doc && ((u.docs[kbase >> 12] >> ((kbase >> 7) & 31)) & 1u);
+#pragma unroll 1
+        for (int x = 0; x < 128; x += 32) {
+            const int a = min(max(lo - kbase - x, 0), 32), z = min(max(hi - kbase - x, 0), 32);
+            uint32_t seen = z > a ? (0xffffffffu >> (32 - z)) & (0xffffffffu << a) : 0u, pk[16];
+            if (docs)
+                for (uint32_t left = seen; left; left &= left - 1u)
+                    if (p.k_doc[u.sq.k0 + kbase + x + __ffs(left) - 1] != qdoc) seen &= ~(left & (~left + 1u));
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 16; q++) pk[q] = ((seen >> (2 * q)) & 1u ? 0x3f80u : 0u) | ((seen >> (2 * q + 1)) & 1u ? 0x3f800000u : 0u);
+            tmem_st16(mine + 128 * buf + x / 2, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_if(&p_full[buf], lane == 0);
+    }
+    // The group of the last tile has seen its S, so that pv_done below is in that tile's phase or past it.
+    const int last = T + u.n - 1;
+    mbar_arrive_if(&e_bar[e], lane == 0);
+    ok = mbar_wait(&e_bar[e], U & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    ok = mbar_wait(&pv_done[last % NS], (last / NS) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    tc_fence_after();
+    const float inf = u.stage == 2 ? INFINITY : -INFINITY;
+    const long at = row * p.nh + head + (p.nsplit > 1 ? (long)u.split * p.q_rows * p.nh : 0);
+#pragma unroll 1
+    for (int c = 0; c < Cfg::OC; c += 16) {
+        uint32_t o[16], hit = 0u;
+        tmem_ld16(mine + Cfg::T_O + wg * Cfg::OC + c, o);
+        tmem_ld_wait();
+        reg_fence<16>(o);
+#pragma unroll
+        for (int q = 0; q < 16; q++) hit |= live && __uint_as_float(o[q]) > 0.f ? 1u << q : 0u;
+        for (; hit; hit &= hit - 1u) {
+            const int ch = u.half * 256 + wg * Cfg::OC + c + __ffs(hit) - 1;
+            if (p.nsplit > 1) {
+                p.part_o[at * p.hd + ch] += inf;
+            } else {
+                bf16_t* out = (bf16_t*)p.out + row * p.ldo + (long)head * p.hd;
+                stf(out, ch, ldf(out, ch) + inf);
+            }
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncwarp();
+    mbar_arrive_if(o_empty, lane == 0);
+    return true;
 }
 
 // The score's parts that a kernel is compiled for; AMT_ANY decides at run time. The softmax is long straight code, and what
@@ -351,10 +374,10 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         if (!mbar_wait(&unit_full[i & 1], (i >> 1) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) return nullptr;
         return units[i & 1].stop ? nullptr : &units[i & 1];
     };
-    // Whether V of key tile kt of a unit is cleaned: rows past the sequence's end that are other sequences' (past the
-    // buffer TMA reads zeros), or a second run.
+    // Whether V of key tile kt of a unit is prepared: rows past the sequence's end that are other sequences' (past the
+    // buffer TMA reads zeros), or a later stage.
     auto guarded = [&](const AmtUnit& u, int kt) {
-        return u.scrub || (kt * 128 + 128 > u.sq.nk && u.sq.k0 + u.sq.nk < p.k_rows);
+        return u.stage != 0 || (kt * 128 + 128 > u.sq.nk && u.sq.k0 + u.sq.nk < p.k_rows);
     };
 
     if (warp < 4) {
@@ -387,7 +410,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     };
                     auto load_k = [&](int x, int kt) { return load(&tmK, k_full, k_empty, Cfg::OFF_R, k_loads, x * 64 * Cfg::UCH, kt); };
                     auto load_v = [&](int x, int kt) { return load(&tmV, v_full, v_empty, Cfg::OFF_V, v_loads, half * 256 + x * 64 * Cfg::UCH, kt); };
-                    TileWalk walk(*un, p.q_doc != nullptr);
+                    TileWalk walk(*un);
                     int kt = walk.next();
                     for (int x = 0; ok && x < KU; x++) ok = load_k(x, kt);
                     for (int j = 0; ok && j < n; j++) {
@@ -423,7 +446,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     d.un = un;
                     d.j = d.x = 0;
                     d.q = false;
-                    d.walk = TileWalk(*un, p.q_doc != nullptr);
+                    d.walk = TileWalk(*un);
                     d.kt = d.walk.next();
                 }
                 return true;
@@ -537,7 +560,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 AmtUnit* un = unit_at(i);
                 if (!un) break;
                 const int n = un->n;
-                TileWalk walk(*un, p.q_doc != nullptr);
+                TileWalk walk(*un);
                 for (int j = 0; ok && j < n; j++, T++) {
                     const int kt = walk.next(), buf = T % NS;
                     const bool clean = guarded(*un, kt);
@@ -545,8 +568,13 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                         const int u = at % RING;
                         if (!(ok = mbar_wait(&v_full[u], (at / RING) & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
                         if (clean) {
+                            bool hit = false;
                             for (int c = 0; c < Cfg::UCH; c++)
-                                guard_chunk(smem + Cfg::OFF_V + u * Cfg::UNIT + c * 16384, un->sq.nk - kt * 128, un->scrub, *un, kt * 128);
+                                hit |= guard_chunk(smem + Cfg::OFF_V + u * Cfg::UNIT + c * 16384, un->sq.nk - kt * 128, un->stage);
+                            if (un->stage == 1 && __any_sync(0xffffffffu, hit) && lane == 0) {
+                                un->bad[kt >> 5] |= 1u << (kt & 31);
+                                un->found = 1;
+                            }
                             fence_proxy_async();
                             __syncwarp();
                         }
@@ -583,16 +611,33 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             for (int i = 0;; i++) {
                 if (i >= 2 && !mbar_wait(&unit_empty[i & 1], ((i >> 1) & 1) ^ 1, EG2_DEV_TIMEOUT_ATTN, abort_flag)) break;
                 AmtUnit& un = units[i & 1];
-                const bool again = i >= 2 && *(volatile int*)&un.retry;
+                int stage = 0;
+                if (i >= 2) {
+                    const volatile AmtUnit& was = un;
+                    stage = was.stage == 0 ? was.retry : was.stage == 1 ? (was.found ? 2 : 0) : was.stage == 2 ? 3 : 0;
+                }
+                const bool again = stage != 0;
                 __syncwarp();
                 if (again || id >= ap.n_units) {
-                    // A unit that met a value that is not finite runs again as it is described; when there is none and
-                    // none is left, an empty unit first, since the other buffer's may still have to run again.
+                    // A unit that met a value that is not finite runs again as it is described, then over the tiles that hold
+                    // some; when there is none and none is left, an empty unit first, since the other buffer's may still
+                    // have to run again.
+                    int n = 0;
+                    if (stage == 1)
+                        for (int w = lane; w < AMT_MASK_WORDS; w += 32) un.bad[w] = 0u;
+                    if (stage == 2) {
+                        for (int w = lane; w < AMT_MASK_WORDS; w += 32) {
+                            const uint32_t v = un.bad[w] ? un.visit[w] & un.bad[w] : 0u;
+                            un.visit[w] = v;
+                            n += __popc(v);
+                        }
+                        n = __reduce_add_sync(0xffffffffu, n);
+                    }
                     if (lane == 0) {
                         un.stop = !again && idle;
-                        un.scrub = again;
-                        un.retry = 0;
-                        un.n_bad = un.masked = 0;
+                        un.stage = stage;
+                        un.retry = un.masked = un.found = 0;
+                        if (stage == 2) un.n = n, un.sparse = 1;
                         if (!again) un.n = un.rows = 0;
                         if (!again && !idle) un.visit[0] = 0u;
                     }
@@ -724,7 +769,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     un.n = n;
                     un.first = first_tile;
                     un.down = min(max(down_to + 1 - first_tile, 0), n);
-                    un.stop = un.scrub = un.retry = un.masked = un.n_bad = 0;
+                    un.sparse = p.q_doc != nullptr;
+                    un.stop = un.stage = un.retry = un.masked = un.found = 0;
                 }
                 __syncwarp();
                 mbar_arrive(&unit_full[i & 1]);
@@ -776,6 +822,13 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             AmtUnit* un = unit_at(i);
             if (!un) break;
             const int n = un->n;
+            if (un->stage >= 2) {
+                if (!(ok = masked_count_unit<HD>(ap, *un, tmem, T, U, s_full, p_full, pv_done, o_empty, e_bar, abort_flag))) break;
+                T += n;
+                U++;
+                if (lane == 0) mbar_arrive(&unit_empty[i & 1]);
+                continue;
+            }
             const bool live = r < un->rows;
             const bool warp_live = 32 * e < un->rows;
             const int tok = un->t0 + r / ap.Gt, head = un->head0 + r % ap.Gt;
@@ -805,7 +858,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             float m = AMT_NONE, l = 0.f;  // the row's maximum at this group's last tile, and its part of the sum in units of 2^m
             bool any_masked = false;
             if (n > 0) {
-                TileWalk walk(*un, p.q_doc != nullptr);
+                TileWalk walk(*un);
                 // The keys that some and that every row of the warp sees.
                 const int some_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : INT_MAX);
                 const int some_hi = __reduce_max_sync(0xffffffffu, lo < hi ? hi : 0);
@@ -902,11 +955,16 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                                         tmem_ld16(ts + c, o);
                                         tmem_ld_wait();
                                         reg_fence<16>(o);
+                                        if (near_ok) {
 #pragma unroll
-                                        for (int q = 0; q < 16; q++) {
-                                            const float x = __uint_as_float(o[q]), y = x * x;
-                                            const float near = x * fmaf(fmaf(fmaf(fmaf(y, c4, c3), y, c2), y, c1), y, c0);
-                                            o[q] = __float_as_uint(y <= near_max ? near : cap2 * tanh_any(x * a));
+                                            for (int q = 0; q < 16; q++) {
+                                                const float x = __uint_as_float(o[q]), y = x * x;
+                                                const float near = x * fmaf(fmaf(fmaf(fmaf(y, c4, c3), y, c2), y, c1), y, c0);
+                                                o[q] = __float_as_uint(y <= near_max ? near : cap2 * tanh_far(x * a));
+                                            }
+                                        } else {
+#pragma unroll
+                                            for (int q = 0; q < 16; q++) o[q] = __float_as_uint(cap2 * tanh_any(__uint_as_float(o[q]) * a));
                                         }
                                         tmem_st16(ts + c, o);
                                     }
@@ -1102,21 +1160,8 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     __syncwarp();
                     mbar_arrive_if(o_empty, lane == 0);
                 }
-                if (!un->scrub) {
-                    if (__any_sync(0xffffffffu, live && odd != 0.f) && *(volatile int*)&un->masked && lane == 0) *(volatile int*)&un->retry = 1;
-                } else {
-                    bool sees_bad = un->n_bad > AMT_BAD;
-                    for (int x = 0; x < min(un->n_bad, AMT_BAD); x++) {
-                        const int key = un->bad[x];
-                        sees_bad |= key >= lo && key < hi && (!p.q_doc || p.k_doc[un->sq.k0 + key] == qdoc);
-                    }
-                    uint32_t rows = __ballot_sync(0xffffffffu, live && sees_bad);
-                    while (rows) {
-                        const int b = __ffs(rows) - 1;
-                        rows &= rows - 1;
-                        masked_row_again<HD>(p, *un, 32 * e + b, ap.Gt, ch0, ch0 + Cfg::OC);
-                    }
-                }
+                if (un->stage == 0 && __any_sync(0xffffffffu, live && odd != 0.f) && *(volatile int*)&un->masked && lane == 0)
+                    *(volatile int*)&un->retry = 1;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&unit_empty[i & 1]);

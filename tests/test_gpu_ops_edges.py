@@ -61,3 +61,92 @@ def test_capped_scores_near_and_far_from_the_cap(dtype, nh, nkv, hd, nq, scale, 
     q, k, v = normal(54, nq, nh, hd, dtype=dtype), normal(55, 333, nkv, hd, dtype=dtype), normal(56, 333, nkv, hd, dtype=dtype)
     opt = dict(scale=scale, softcap=softcap)
     check_attention(q, k, v, ql, kl, attend(q, k, v, ql, kl, **opt), **opt)
+
+
+# ---- values that are not finite ---------------------------------------------------------------------------
+def places(ql, kl):
+    """Place of each query row among its sequence's keys, and its sequence."""
+    at = [(nk - nq + t, b) for b, (nq, nk) in enumerate(zip(ql, kl)) for t in range(nq)]
+    return torch.tensor([a for a, _ in at]).cuda(), torch.tensor([b for _, b in at]).cuda()
+
+
+BF16_HEADS = [(BF16, 4, 2, 64), (BF16, 2, 1, 128), (BF16, 4, 2, 256), (BF16, 4, 1, 512), (BF16, 3, 1, 128), (BF16, 3, 3, 80)]
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("ql,kl", [([390], [390]), ([5, 3], [200, 700]), ([60], [4000]), ([40, 300], [900, 300])])
+def test_any_number_of_hidden_values_may_not_be_finite(dtype, nh, nkv, hd, ql, kl):
+    """Dozens of NaN and infinite rows of V in a hidden document, and past a causal bound: the other rows keep their bits."""
+    q, k, v = normal(31, sum(ql), nh, hd, scale=2.0, dtype=dtype), normal(32, sum(kl), nkv, hd, dtype=dtype), normal(33, sum(kl), nkv, hd, dtype=dtype)
+    n = sum(kl)
+    j = torch.arange(n)
+    k_doc = ((j % 9 == 4) | ((j > n // 2) & (j < n // 2 + 40))).to(torch.int32).cuda()
+    q_doc = torch.zeros(sum(ql), dtype=torch.int32, device="cuda")
+    opt = dict(scale=hd ** -0.5, softcap=30.0, q_doc=q_doc, k_doc=k_doc)
+    clean = attend(q, k, v, ql, kl, **opt)
+    check_attention(q, k, v, ql, kl, clean, **opt)
+    bad = v.clone()
+    bad[k_doc == 1] = math.nan
+    bad[(k_doc == 1) & (j.cuda() % 2 == 0)] = math.inf
+    got = attend(q, k, bad, ql, kl, **opt)
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
+    # the last 70 keys of every sequence, seen by its last queries alone
+    opt = dict(scale=hd ** -0.5, causal=True)
+    clean = attend(q, k, v, ql, kl, **opt)
+    bad, place, seq = v.clone(), *places(ql, kl)
+    sees = torch.zeros(sum(ql), dtype=torch.bool, device="cuda")
+    for b, end in enumerate(np.cumsum(kl)):
+        bad[int(end) - 70 : int(end)] = math.nan
+        sees |= (seq == b) & (place >= kl[b] - 70)
+    out, lse = attend(q, k, bad, ql, kl, **opt)
+    assert torch.equal(out[~sees], clean[0][~sees]) and torch.equal(lse, clean[1])
+    assert not bool(torch.isfinite(out[sees]).any())
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("ql,kl", [([390], [390]), ([3], [700]), ([2], [5003]), ([60], [4000]), ([17, 200], [1500, 200])])
+@pytest.mark.parametrize("window", [-1, 60])
+def test_visible_infinities_keep_their_sign_and_channel(dtype, nh, nkv, hd, ql, kl, window):
+    """A channel that meets one kind of infinity becomes it, one that meets both or a NaN becomes NaN, for the rows that see
+    the key; all else keeps its bits."""
+    q, k, v = normal(41, sum(ql), nh, hd, scale=2.0, dtype=dtype), normal(42, sum(kl), nkv, hd, dtype=dtype), normal(43, sum(kl), nkv, hd, dtype=dtype)
+    opt = dict(scale=hd ** -0.5, causal=True, window=window)
+    clean = attend(q, k, v, ql, kl, **opt)
+    bad, place, seq = v.clone(), *places(ql, kl)
+    want = clean[0].double()
+    G = nh // nkv
+    for b, (end, n) in enumerate(zip(np.cumsum(kl), kl)):
+        for back, ch, e in ((1, 0, math.inf), (2, 0, math.inf), (2, 1, -math.inf), (3, 2, math.nan), (40, 3, math.inf), (50, 3, -math.inf),
+                            (30, hd - 1, -math.inf), (130, hd // 2, math.inf)):
+            key = n - back
+            bad[int(end) - back, 0, ch] = e
+            rows = (seq == b) & (place >= key)
+            if window >= 0:
+                rows &= place - key <= window
+            want[rows, :G, ch] += e  # the first K/V head's query heads
+    out, lse = attend(q, k, bad, ql, kl, **opt)
+    kept = torch.isfinite(want)
+    assert torch.equal(out[kept], clean[0][kept]) and torch.equal(lse, clean[1])
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out[torch.isinf(want)].double(), want[torch.isinf(want)])
+    assert L.load().eg2_device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd,nq", [h + (64,) for h in BF16_HEADS] + [(BF16, 1, 1, 64, 20_000), (BF16, 1, 1, 128, 20_000)])
+def test_a_value_that_is_not_finite_in_a_long_sequence(dtype, nh, nkv, hd, nq):
+    """200,000 keys, one of them infinite, one NaN in one channel, one NaN and hidden from all but the last query; with the key axis
+    split and whole: no wait runs out."""
+    n = 200_000
+    q, k, v = normal(44, nq, nh, hd, scale=2.0, dtype=dtype), normal(45, n, nkv, hd, dtype=dtype), normal(46, n, nkv, hd, dtype=dtype)
+    opt = dict(scale=hd ** -0.5, causal=True)
+    clean = attend(q, k, v, [nq], [n], **opt)
+    v[777] = math.inf * v[777].sign()
+    v[n - 30, :, 5] = math.nan
+    v[n - 1] = math.nan
+    out, lse = attend(q, k, v, [nq], [n], **opt)
+    torch.cuda.synchronize()
+    assert L.load().eg2_device_status() == 0
+    assert torch.equal(lse, clean[1])
+    assert bool(torch.isnan(out[-1]).all()) and bool(torch.isnan(out[nq - 30 :, :, 5]).all())
+    sign = v[777].repeat_interleave(nh // nkv, 0)
+    assert torch.equal(out[: nq - 30], sign.expand(nq - 30, nh, hd))
