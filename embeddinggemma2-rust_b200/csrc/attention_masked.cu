@@ -5,8 +5,8 @@
 //   out_i   = sum_j softmax_j(x(i, j)) v_j over the keys j that i may see,  lse_i = log sum_j exp x(i, j)
 //
 // i and j are places within the sequence; the queries are its last places. What i may see is an interval
-// [lo, hi) of keys -- the window and the causal or prefix bound -- less the keys of other documents. A row that
-// sees nothing gets out = 0, lse = -inf. Keys that a row may not see contribute nothing whatever they hold.
+// [lo, hi) of keys -- the window and the causal or prefix bound -- less the keys of other documents and those with a
+// bias of -infinity. A row that sees nothing gets out = 0, lse = -inf. Keys that a row may not see contribute nothing whatever they hold.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -58,8 +58,12 @@ EG2_DEV void masked_range(const MaskedParams& p, const MaskedSeq& s, int i, int&
 }
 
 // A distance bias as it is used: finite ones are at least -1e30, so that a row whose keys all have the type's lowest value
-// keeps its softmax (the log2 domain of the tensor-core form would overflow), -infinity hides a key.
+// keeps its softmax (the log2 domain of the tensor-core form would overflow). -infinity is a mask: it is not added but tested,
+// since a key that it hides may have a score that is not finite.
 EG2_DEV float masked_bias(float b) { return b < -1e30f && b > -INFINITY ? -1e30f : b; }
+EG2_DEV float masked_table(const MaskedParams& p, int head, int apart) {
+    return masked_bias(p.table[(long)head * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]);
+}
 
 // ---------------------------------------------------------------------------------------------
 // CUDA cores, f32 arithmetic. A block takes 16 RPT rows (row r = token r / G, head r % G of the K/V head's G
@@ -237,8 +241,12 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
                 float v = p.softcap > 0.f ? p.softcap * tanhf(s[i][x] * inv_cap) : s[i][x] * p.scale;
                 const int apart = key - place[i];
                 if (p.slopes) v -= p.slopes[head[i]] * fabsf((float)apart);
-                if (p.table) v += masked_bias(p.table[(long)head[i] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]);
-                const bool seen = key >= lo[i] && key < hi[i] && (!p.k_doc || docs[tx + 16 * x] == qdoc[i]);
+                bool seen = key >= lo[i] && key < hi[i] && (!p.k_doc || docs[tx + 16 * x] == qdoc[i]);
+                if (p.table) {
+                    const float bias = masked_table(p, head[i], apart);
+                    seen = seen && bias != -INFINITY;
+                    v += bias;
+                }
                 hidden |= !seen;
                 s[i][x] = seen ? v : -INFINITY;
                 top = fmaxf(top, s[i][x]);

@@ -266,21 +266,31 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
 #pragma unroll
             for (int x = 0; x < 8; x++) v[x] = fmaf(-slope[x >> 2], fabsf((float)(col0 + 8 * ((x >> 1) & 1) + (x & 1) - place[x >> 2])), v[x]);
         }
+        uint32_t unseen = 0u;  // of this thread's eight scores
         if (p.table) {
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                const int apart = col0 + 8 * ((x >> 1) & 1) + (x & 1) - place[x >> 2];
-                v[x] += masked_bias(p.table[(long)head[x >> 2] * (2 * p.radius + 1) + p.radius + min(max(apart, -p.radius), p.radius)]) * AMT_LOG2E;
+                const float bias = masked_table(p, head[x >> 2], col0 + 8 * ((x >> 1) & 1) + (x & 1) - place[x >> 2]);
+                v[x] = fmaf(bias, AMT_LOG2E, v[x]);
+                unseen |= bias == -INFINITY ? 1u << x : 0u;
             }
         }
-        bool hidden = false;  // some key is hidden from some row of this thread
         if (p.k_doc || key0 < all_lo || key0 + 16 > all_hi) {
 #pragma unroll
             for (int x = 0; x < 8; x++) {
                 const int key = col0 + 8 * ((x >> 1) & 1) + (x & 1), y = x >> 2;
                 const bool seen = key >= lo[y] && key < hi[y] && (!p.k_doc || ids[x & 3] == qdoc[y]);
-                hidden |= !seen && (lane >> 2) + 8 * y < rows;
-                v[x] = seen ? v[x] : -INFINITY;
+                unseen |= seen ? 0u : 1u << x;
+            }
+        }
+        bool hidden = false;  // some key is hidden from some row
+        if (unseen) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                if ((unseen >> x) & 1u) {
+                    v[x] = -INFINITY;
+                    hidden |= (lane >> 2) + 8 * (x >> 2) < rows;
+                }
             }
         }
         float top[2];

@@ -229,7 +229,8 @@ EG2_DEV bool masked_count_unit(const AmtParams& ap, const AmtUnit& u, uint32_t t
     const int t = u.t0 + r / ap.Gt, head = u.head0 + r % ap.Gt;
     const long row = u.sq.q0 + t;
     int lo = 0, hi = 0;
-    if (live) masked_range(p, u.sq, u.sq.nk - u.sq.nq + t, lo, hi);
+    const int place = u.sq.nk - u.sq.nq + t;
+    if (live) masked_range(p, u.sq, place, lo, hi);
     const int qdoc = live && p.q_doc ? p.q_doc[row] : 0;
     TileWalk walk(u);
     bool ok = true;
@@ -244,9 +245,12 @@ EG2_DEV bool masked_count_unit(const AmtParams& ap, const AmtUnit& u, uint32_t t
         for (int x = 0; x < 128; x += 32) {
             const int a = min(max(lo - kbase - x, 0), 32), z = min(max(hi - kbase - x, 0), 32);
             uint32_t seen = z > a ? (0xffffffffu >> (32 - z)) & (0xffffffffu << a) : 0u, pk[16];
-            if (docs)
-                for (uint32_t left = seen; left; left &= left - 1u)
-                    if (p.k_doc[u.sq.k0 + kbase + x + __ffs(left) - 1] != qdoc) seen &= ~(left & (~left + 1u));
+            if (docs || p.table)
+                for (uint32_t left = seen; left; left &= left - 1u) {
+                    const int key = kbase + x + __ffs(left) - 1;
+                    if ((docs && p.k_doc[u.sq.k0 + key] != qdoc) || (p.table && masked_table(p, head, key - place) == -INFINITY))
+                        seen &= ~(left & (~left + 1u));
+                }
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 16; q++) pk[q] = ((seen >> (2 * q)) & 1u ? 0x3f80u : 0u) | ((seen >> (2 * q + 1)) & 1u ? 0x3f800000u : 0u);
@@ -326,6 +330,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
     uint64_t* drain = t_bar + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* table_hides = abort_flag + 1;  // [2], by build: the staged table holds -infinity
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -353,6 +358,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             mbar_init(&v_empty[x], 1);
         }
         *abort_flag = 0;
+        table_hides[0] = table_hides[1] = 0;
         fence_mbarrier_init();
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
@@ -816,7 +822,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const float c0 = AMT_T0 * a * cap2, c1 = AMT_T1 * a * a * a * cap2, c2 = AMT_T2 * (a * a) * (a * a) * a * cap2,
                     c3 = AMT_T3 * (a * a * a) * (a * a * a) * a * cap2, c4 = AMT_T4 * (a * a * a) * (a * a * a) * (a * a * a) * cap2;
         int T = 0, U = 0, tab_head = -1, builds = 0;
-        bool ok = true;
+        bool ok = true, hides = false;
 
         for (int i = 0; ok; i++) {
             AmtUnit* un = unit_at(i);
@@ -845,13 +851,17 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_bar[0]);
                 if (!(ok = mbar_wait(&t_bar[0], builds & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                if (s_tid == 0) table_hides[(builds + 1) & 1] = 0;  // the build before has been read, the next one waits for t_bar[0]
                 for (int x = s_tid; x < ap.Gt * tab_ld; x += 256) {
                     const int hh = x / tab_ld, c = min(max(x % tab_ld - 128, 0), 2 * p.radius);
-                    table[x] = masked_bias(p.table[(long)(tab_head + hh) * (2 * p.radius + 1) + c]) * AMT_LOG2E;
+                    const float b = masked_bias(p.table[(long)(tab_head + hh) * (2 * p.radius + 1) + c]);
+                    table[x] = b * AMT_LOG2E;
+                    if (b == -INFINITY) table_hides[builds & 1] = 1;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_bar[1]);
                 if (!(ok = mbar_wait(&t_bar[1], builds & 1, EG2_DEV_TIMEOUT_ATTN, abort_flag))) break;
+                hides = table_hides[builds & 1];
                 builds++;
             }
             const float* my_table = table + (r % ap.Gt) * tab_ld;
@@ -882,9 +892,9 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     const uint32_t ts = tmem + 128 * buf + lane_off;
                     const bool sees = kbase < some_hi && kbase + NC > some_lo;
                     const bool docs = p.q_doc && ((un->docs[kbase >> 12] >> ((kbase >> 7) & 31)) & 1u);
-                    const bool full = !docs && kbase >= all_lo && kbase + NC <= all_hi;
+                    const bool full = !docs && !(tables && hides) && kbase >= all_lo && kbase + NC <= all_hi;
                     any_masked |= !full;
-                    uint32_t same[4] = {~0u, ~0u, ~0u, ~0u};  // columns of this row's document
+                    uint32_t same[4] = {~0u, ~0u, ~0u, ~0u};  // columns of this row's document that no bias hides
                     if (docs && sees) {
                         // The rows of a warp are of few documents, mostly one: a ballot per document and 32 columns.
                         uint32_t left = __ballot_sync(0xffffffffu, lo < hi);
@@ -899,6 +909,14 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                                 if (qdoc == d) same[x] = cols;
                             }
                         }
+                    }
+                    if (tables && hides && sees) {
+                        const float* tb = my_table + min(max(kbase - place, -p.radius - 128), p.radius) + p.radius + 128;
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+#pragma unroll 1
+                            for (int c = 0; c < 32; c++)
+                                if (tb[32 * x + c] == -INFINITY) same[x] &= ~(1u << c);
                     }
                     if (j + 2 < n) {
                         walk.next();

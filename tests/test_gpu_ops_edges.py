@@ -150,3 +150,47 @@ def test_a_value_that_is_not_finite_in_a_long_sequence(dtype, nh, nkv, hd, nq):
     assert bool(torch.isnan(out[-1]).all()) and bool(torch.isnan(out[nq - 30 :, :, 5]).all())
     sign = v[777].repeat_interleave(nh // nkv, 0)
     assert torch.equal(out[: nq - 30], sign.expand(nq - 30, nh, hd))
+
+
+# ---- biases of minus infinity ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("ql,kl", [([150], [150]), ([3], [150]), ([70, 330], [70, 330]), ([2], [5003]), ([100], [4000])])
+@pytest.mark.parametrize("heads", ["all", "first"])
+def test_biases_of_minus_infinity_hide_keys(dtype, nh, nkv, hd, ql, kl, heads):
+    """A bias of -infinity is a mask: what keys hold under it (NaN, infinities, in K or in V) reaches no row, to the bit."""
+    R = 9
+    table = normal(11, nh, 2 * R + 1, scale=2.0)
+    hide = slice(0, nh if heads == "all" else 1)
+    table[hide, 2 * R] = -math.inf     # keys R and more ahead
+    table[hide, : R - 4] = -math.inf   # keys 5 and more behind
+    table[hide, R + 2] = -math.inf     # and one in between
+    q, k, v = normal(12, sum(ql), nh, hd, scale=2.0, dtype=dtype), normal(13, sum(kl), nkv, hd, dtype=dtype), normal(14, sum(kl), nkv, hd, dtype=dtype)
+    opt = dict(scale=hd ** -0.5, softcap=20.0, table=table)
+    clean = attend(q, k, v, ql, kl, **opt)
+    check_attention(q, k, v, ql, kl, clean, **opt)
+    place, seq = places(ql, kl)
+    start = torch.tensor(np.cumsum([0] + kl)[:-1]).cuda()
+    for what, bad in (("v", math.nan), ("v", -math.inf), ("k", math.nan), ("k", math.inf)):
+        kk, vv = k.clone(), v.clone()
+        sees = torch.zeros(sum(ql), nh, dtype=torch.bool, device="cuda")
+        for b, n in enumerate(kl):
+            for key in {0, n // 2, n - 1}:
+                (vv if what == "v" else kk)[int(start[b]) + key] = bad
+                bias = table.T[(key - place).clamp(-R, R) + R]  # [rows, nh]
+                sees |= (seq == b)[:, None] & (bias != -math.inf)
+        out, lse = attend(q, kk, vv, ql, kl, **opt)
+        assert torch.equal(out[~sees], clean[0][~sees]) and torch.equal(lse[~sees], clean[1][~sees])
+        if what == "v":
+            assert not bool(torch.isfinite(out[sees]).any())
+    assert L.load().eg2_device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("ql,kl", [([150], [150]), ([3], [150]), ([2], [5003]), ([100], [4000])])
+def test_rows_that_a_bias_hides_whole_are_empty(dtype, nh, nkv, hd, ql, kl):
+    table = torch.zeros(nh, 5, device="cuda")
+    table[-1] = -math.inf
+    q, k, v = normal(15, sum(ql), nh, hd, dtype=dtype), normal(16, sum(kl), nkv, hd, dtype=dtype), normal(17, sum(kl), nkv, hd, dtype=dtype)
+    k[:, -1, ::3], v[:, -1, ::2] = math.nan, math.inf
+    out, lse = attend(q, k, v, ql, kl, scale=hd ** -0.5, table=table)
+    assert bool((out[:, -1] == 0).all()) and bool((lse[:, -1] == -math.inf).all())
