@@ -27,7 +27,9 @@ struct MaskedParams {
     int n_seq, max_q, max_k, nh, nkv, hd, G, window, causal, radius;
     int nsplit, part;  // the key axis in nsplit parts of `part` key tiles each
     float scale, softcap;
-    float *part_o, *part_lse;  // nsplit > 1: [nsplit][q_rows][nh][hd] and [nsplit][q_rows][nh]
+    float* part_o;   // nsplit > 1: [nsplit][q_rows][nh][hd]
+    float2* part_ml; // and [nsplit][q_rows][nh]: a part's maximum and its sum in units of that
+    int log2_parts;  // maxima in the log2 domain (the forms for bf16)
 };
 
 // One sequence: its rows, clamped to the buffers and to the stated maxima whatever the offsets hold.
@@ -314,17 +316,16 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
         if (rr >= n_rows) continue;
         const long row = sq.q0 + rr / p.G;
         const float inv = l[i] > 0.f ? 1.f / l[i] : l[i] == 0.f ? 0.f : l[i];  // NaN stays
-        const float lse = l[i] == 0.f ? -INFINITY : m[i] + logf(l[i]);
         if (p.nsplit > 1) {
             const long at = ((long)split * p.q_rows + row) * p.nh + head[i];
-            if (tx == 0) p.part_lse[at] = lse;
+            if (tx == 0) p.part_ml[at] = make_float2(m[i], l[i]);
 #pragma unroll
             for (int c = 0; c < NCH; c++)
 #pragma unroll
                 for (int x = 0; x < 4; x++)
                     if (c * 64 + tx * 4 + x < p.hd) p.part_o[at * p.hd + c * 64 + tx * 4 + x] = o[c][i][x] * inv;
         } else {
-            if (tx == 0 && p.lse) p.lse[row * p.nh + head[i]] = lse;
+            if (tx == 0 && p.lse) p.lse[row * p.nh + head[i]] = l[i] == 0.f ? -INFINITY : m[i] + logf(l[i]);
             T* orow = (T*)p.out + row * p.ldo + (long)head[i] * p.hd;
 #pragma unroll
             for (int c = 0; c < NCH; c++)
@@ -338,7 +339,15 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
 #include "attention_masked_tc.cuh"
 #include "attention_masked_few.cuh"
 
-// Joins the parts of a split key axis: out = sum_s exp(lse_s - lse) o_s, in part order. A block per (sequence, query, head),
+EG2_DEV float masked_part_weight(const MaskedParams& p, float2 ml, float base) {
+    return ml.y == 0.f ? 0.f : ml.y * (p.log2_parts ? ex2_approx(ml.x - base) : expf(ml.x - base));
+}
+EG2_DEV float masked_part_lse(const MaskedParams& p, float base, float total) {
+    return total == 0.f ? -INFINITY : p.log2_parts ? (base + log2f(total)) * 0.6931471805599453f : base + logf(total);
+}
+
+// Joins the parts of a split key axis: out = sum_s w_s o_s / sum_s w_s with w_s = l_s exp(m_s - max m), in part order. Maximum and sum
+// come apart: of m + log l in 32 bits little is left of the sum where the maximum is large. A block per (sequence, query, head),
 // two groups of 128 threads that take every other part; the parts' results are on their way while the weights are
 // worked out. Bound by latency: few rows, their parts read once.
 template <typename T>
@@ -364,8 +373,8 @@ __global__ void __launch_bounds__(256) attention_masked_join_kernel(const Masked
     }
     float top = -INFINITY;
     for (int s = threadIdx.x; s < p.nsplit; s += 256) {
-        weight[s] = p.part_lse[s * step + item];
-        top = fmaxf(top, weight[s]);
+        const float2 ml = p.part_ml[s * step + item];
+        top = fmaxf(top, ml.y == 0.f ? -INFINITY : ml.x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -374,7 +383,7 @@ __global__ void __launch_bounds__(256) attention_masked_join_kernel(const Masked
 #pragma unroll
     for (int x = 0; x < 8; x++) top = fmaxf(top, red[x]);
     const float base = top == -INFINITY ? 0.f : top;
-    for (int s = threadIdx.x; s < p.nsplit; s += 256) weight[s] = expf(weight[s] - base);
+    for (int s = threadIdx.x; s < p.nsplit; s += 256) weight[s] = masked_part_weight(p, p.part_ml[s * step + item], base);
     __syncthreads();
     float total = 0.f;
     for (int s = 0; s < p.nsplit; s++) total += weight[s];  // the same sum in every thread
@@ -407,7 +416,7 @@ __global__ void __launch_bounds__(256) attention_masked_join_kernel(const Masked
             const int c = c0 + 128 * x;
             if (c < p.hd) stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, (sum[x] + second[c]) * inv);
         }
-        if (c0 == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+        if (c0 == 0 && p.lse) p.lse[item] = masked_part_lse(p, base, total);
     }
 }
 
@@ -428,11 +437,11 @@ __global__ void __launch_bounds__(256) attention_masked_join_rows_kernel(const M
     const MaskedSeq sq = masked_seq(p, b);
     if (t >= sq.nq) return;
     const long row = sq.q0 + t, item = row * p.nh + h, step = p.q_rows * p.nh;
-    const float lse = lane < p.nsplit ? p.part_lse[lane * step + item] : -INFINITY;
-    float top = lse;
+    const float2 ml = lane < p.nsplit ? p.part_ml[lane * step + item] : make_float2(0.f, 0.f);
+    float top = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top, mine = expf(lse - base);
+    const float base = top == -INFINITY ? 0.f : top, mine = masked_part_weight(p, ml, base);
     float w[JOIN_PARTS], total = 0.f;
 #pragma unroll
     for (int s = 0; s < JOIN_PARTS; s++) total += w[s] = __shfl_sync(0xffffffffu, mine, s);
@@ -446,7 +455,7 @@ __global__ void __launch_bounds__(256) attention_masked_join_rows_kernel(const M
         for (int s = 0; s < JOIN_PARTS; s++) sum = fmaf(w[s], o[s], sum);
         stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, sum * inv);
     }
-    if (lane == 0 && p.lse) p.lse[item] = total == 0.f ? -INFINITY : base + logf(total);
+    if (lane == 0 && p.lse) p.lse[item] = masked_part_lse(p, base, total);
 }
 
 template <typename T, int NCH, int RPT>
@@ -549,6 +558,11 @@ static MaskedPlan masked_plan(const eg2_masked_attention* a) {
     return r;
 }
 
+// Workspace: the parts' results, then their maxima and sums, at an even number of floats.
+static int64_t masked_part_ml_at(const eg2_masked_attention* a, int nsplit) {
+    return ((int64_t)nsplit * a->q_rows * a->nh * a->hd + 1) / 2 * 2;
+}
+
 static bool masked_valid(const eg2_masked_attention* a) {
     if (!a || (a->kind != EG2_F32 && a->kind != EG2_BF16)) return false;
     if (a->n_seq < 0 || a->max_q < 0 || a->max_k < 0 || a->q_rows < 0 || a->k_rows < 0) return false;
@@ -572,7 +586,7 @@ extern "C" {
 int64_t eg2_attention_masked_workspace(const eg2_masked_attention* a) {
     if (!eg2::masked_valid(a)) return EG2_ERR_INVALID;
     const int n = eg2::masked_plan(a).nsplit;
-    return n > 1 ? (int64_t)n * a->q_rows * a->nh * (a->hd + 1) * 4 : 0;
+    return n > 1 ? eg2::masked_part_ml_at(a, n) * 4 + (int64_t)n * a->q_rows * a->nh * 8 : 0;
 }
 
 int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -582,7 +596,7 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
     if (!a->q || !a->out || !a->q_off || !a->k_off || (a->k_rows > 0 && (!a->k || !a->v))) return EG2_ERR_INVALID;
     MaskedParams p{a->q, a->k, a->v, a->out, a->lse, a->ldq, a->ldk, a->ldv, a->ldo, a->q_off, a->k_off, a->prefix_len, a->q_doc,
                    a->k_doc, a->slopes, a->dist_bias, a->q_rows, a->k_rows, a->n_seq, a->max_q, a->max_k, a->nh, a->nkv, a->hd,
-                   a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, 0, a->scale, a->softcap, nullptr, nullptr};
+                   a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, 0, a->scale, a->softcap, nullptr, nullptr, 0};
     cudaStream_t s = (cudaStream_t)stream;
     const MaskedPlan plan = masked_plan(a);
     p.nsplit = plan.nsplit;
@@ -590,7 +604,8 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
     if (p.nsplit > 1) {
         if (!workspace || workspace_bytes < eg2_attention_masked_workspace(a) || (uintptr_t)workspace % 16) return EG2_ERR_INVALID;
         p.part_o = (float*)workspace;
-        p.part_lse = p.part_o + (long)p.nsplit * p.q_rows * p.nh * p.hd;
+        p.part_ml = (float2*)(p.part_o + masked_part_ml_at(a, p.nsplit));
+        p.log2_parts = plan.tc;
     }
     int rc;
     if (plan.few) {

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
     const int words = (last - first + 31) / 32;
     if (p.nsplit > 1 && first == last) {  // a short sequence's later parts: their slot on the SM is wanted
         if (half == 0 && (int)threadIdx.x < rows)
-            p.part_lse[((long)split * p.q_rows + sq.q0 + threadIdx.x / p.G) * p.nh + g * p.G + threadIdx.x % p.G] = -INFINITY;
+            p.part_ml[((long)split * p.q_rows + sq.q0 + threadIdx.x / p.G) * p.nh + g * p.G + threadIdx.x % p.G] = make_float2(AMT_NONE, 0.f);
         return;
     }
 
@@ -433,11 +433,10 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
             if (ch < p.hd) stf((bf16_t*)p.out + row * p.ldo + (long)h * p.hd, ch, ll == 0.f ? 0.f : a * inv);
         }
         if (c == 0 && half == 0) {
-            const float lse = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
             if (p.nsplit > 1)
-                p.part_lse[(long)split * p.q_rows * p.nh + at] = lse;
+                p.part_ml[(long)split * p.q_rows * p.nh + at] = make_float2(mm, ll);
             else if (p.lse)
-                p.lse[at] = lse;
+                p.lse[at] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
         }
     }
 }

@@ -1121,11 +1121,10 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                 const long row = un->sq.q0 + tok;
                 const long at = row * p.nh + head + (p.nsplit > 1 ? (long)un->split * p.q_rows * p.nh : 0);
                 if (live && un->half == 0 && wg == 0) {
-                    const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                     if (p.nsplit > 1)
-                        p.part_lse[at] = lse;
+                        p.part_ml[at] = make_float2(m, l);
                     else if (p.lse)
-                        p.lse[at] = lse;
+                        p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                 }
                 const int ch0 = un->half * 256 + wg * Cfg::OC;
                 const uint32_t to = tmem + Cfg::T_O + wg * Cfg::OC + lane_off;

@@ -194,3 +194,31 @@ def test_rows_that_a_bias_hides_whole_are_empty(dtype, nh, nkv, hd, ql, kl):
     k[:, -1, ::3], v[:, -1, ::2] = math.nan, math.inf
     out, lse = attend(q, k, v, ql, kl, scale=hd ** -0.5, table=table)
     assert bool((out[:, -1] == 0).all()) and bool((lse[:, -1] == -math.inf).all())
+
+
+# ---- the parts of a split key axis under large biases -----------------------------------------------------
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("nq", [1, 3, 100, 330])
+@pytest.mark.parametrize("bias", [torch.finfo(F32).min, -1e30, -1e6, -1e5, 3e4])
+@pytest.mark.parametrize("docs", [False, True])
+def test_parts_are_weighted_by_their_sums_under_any_bias(dtype, nh, nkv, hd, nq, bias, docs):
+    """All scores equal: every visible key weighs the same, however few of them a part of the key axis holds and however large
+    the bias is that all scores carry. Values rise along the keys, so that a part's wrong share shows."""
+    ql, kl = [nq], [5003]
+    q = torch.zeros(nq, nh, hd, dtype=dtype, device="cuda")
+    k = normal(21, 5003, nkv, hd, dtype=dtype)
+    v = (normal(22, 5003, nkv, hd) + torch.linspace(-2.0, 4.0, 5003).cuda()[:, None, None]).to(dtype)
+    q_doc = k_doc = None
+    if docs:  # visible: the first 40 keys, every 7th up to 3,000, all past 4,900
+        j = torch.arange(5003)
+        k_doc = ((j < 40) | ((j < 3000) & (j % 7 == 0)) | (j > 4900)).to(torch.int32).cuda()
+        q_doc = torch.ones(nq, dtype=torch.int32, device="cuda")
+    got = attend(q, k, v, ql, kl, table=torch.full((nh, 3), bias).cuda(), q_doc=q_doc, k_doc=k_doc)
+    # The weights do not depend on the common bias (in 64 bits, too, the log-sum beside -1e30 would lose the sum).
+    want, wlse, mag, _ = attention_64(q, k, v, ql, kl, q_doc=q_doc, k_doc=k_doc)
+    out, lse = got
+    rel = 2.0**-8 if dtype == BF16 else 2.0**-14  # bf16: the result's rounding; f32: a running sum of 5,003 terms
+    assert bool(((out.double() - want).abs() <= rel * (mag + want.abs())).all())
+    # bias and sum in units of log 2 and back: four roundings of 2^-24
+    bias = max(bias, -1e30)
+    assert bool(((lse.double() - (wlse + bias)).abs() <= 2.0**-22 * abs(bias) + 2.0**-18 * wlse.abs()).all())
