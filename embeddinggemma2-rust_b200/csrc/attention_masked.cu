@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
         bool hidden = false;
 #pragma unroll
         for (int i = 0; i < RPT; i++) {
+            uint32_t unseen = 0u;
             float top = -INFINITY;
 #pragma unroll
             for (int x = 0; x < 4; x++) {
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
                     seen = seen && bias != -INFINITY;
                     v += bias;
                 }
-                hidden |= !seen;
+                unseen |= seen ? 0u : 1u << x;
                 s[i][x] = seen ? v : -INFINITY;
                 top = fmaxf(top, s[i][x]);
             }
@@ -264,6 +265,12 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
                 const float e = expf(s[i][x] - base);
                 sum += e;
                 ps[(ty * RPT + i) * AMS_LD + tx + 16 * x] = e;
+            }
+            if (unseen) {  // -0 marks a hidden key: a weight that has vanished is +0
+                hidden = true;
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if ((unseen >> x) & 1u) ps[(ty * RPT + i) * AMS_LD + tx + 16 * x] = -0.f;
             }
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -293,8 +300,8 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
 #pragma unroll
                         for (int i = 0; i < RPT; i++) {
                             const float pe = e == 0 ? a[i].x : e == 1 ? a[i].y : e == 2 ? a[i].z : a[i].w;
-                            // A hidden key's value may be anything: 0 x NaN must not reach the sum.
-                            if (!decltype(guard)::value || pe != 0.f) {
+                            // A hidden key's value may be anything: 0 x NaN must not reach the sum, of a key that the row sees it must.
+                            if (!decltype(guard)::value || __float_as_uint(pe) != 0x80000000u) {
                                 o[ch][i][0] = fmaf(pe, w.x, o[ch][i][0]);
                                 o[ch][i][1] = fmaf(pe, w.y, o[ch][i][1]);
                                 o[ch][i][2] = fmaf(pe, w.z, o[ch][i][2]);
@@ -339,8 +346,11 @@ __global__ void __launch_bounds__(256, RPT == 2 && NCH <= 4 ? 2 : 1) attention_m
 #include "attention_masked_tc.cuh"
 #include "attention_masked_few.cuh"
 
+// A part that has seen nothing weighs -0 and may hold anything; one whose weight has vanished counts all the same, as its sum may not
+// be finite.
+EG2_DEV bool masked_part_counts(float w) { return __float_as_uint(w) != 0x80000000u; }
 EG2_DEV float masked_part_weight(const MaskedParams& p, float2 ml, float base) {
-    return ml.y == 0.f ? 0.f : ml.y * (p.log2_parts ? ex2_approx(ml.x - base) : expf(ml.x - base));
+    return ml.y == 0.f ? -0.f : ml.y * (p.log2_parts ? ex2_approx(ml.x - base) : expf(ml.x - base));
 }
 EG2_DEV float masked_part_lse(const MaskedParams& p, float base, float total) {
     return total == 0.f ? -INFINITY : p.log2_parts ? (base + log2f(total)) * 0.6931471805599453f : base + logf(total);
@@ -352,7 +362,7 @@ EG2_DEV float masked_part_lse(const MaskedParams& p, float base, float total) {
 // worked out. Bound by latency: few rows, their parts read once.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_masked_join_kernel(const MaskedParams p) {
-    extern __shared__ float weight[];  // [nsplit], then [hd] of the second group
+    extern __shared__ float weight[];  // [nsplit] (-0: nothing seen), then [hd] of the second group
     __shared__ float red[8];
     grid_dep_launch();
     grid_dep_wait();
@@ -394,17 +404,16 @@ __global__ void __launch_bounds__(256) attention_masked_join_kernel(const Masked
     for (int x = 0; x < 4; x++) {
         const int c = c0 + 128 * x;
         if (c >= p.hd) break;
-        // A part that counts nothing may hold anything.
         int s = group;
         if (x == 0) {
 #pragma unroll
             for (int y = 0; y < AHEAD; y++, s += 2)
-                if (s < p.nsplit && weight[s] != 0.f) sum[x] = fmaf(weight[s], early[y], sum[x]);
+                if (s < p.nsplit && masked_part_counts(weight[s])) sum[x] = fmaf(weight[s], early[y], sum[x]);
         }
 #pragma unroll 8
         for (; s < p.nsplit; s += 2) {
             const float w = weight[s];
-            const float o = w != 0.f ? p.part_o[(s * step + item) * p.hd + c] : 0.f;
+            const float o = masked_part_counts(w) ? p.part_o[(s * step + item) * p.hd + c] : 0.f;
             sum[x] = fmaf(w, o, sum[x]);
         }
         if (group) second[c] = sum[x];
@@ -450,7 +459,7 @@ __global__ void __launch_bounds__(256) attention_masked_join_rows_kernel(const M
     for (int c = lane; c < p.hd; c += 32) {
         float o[JOIN_PARTS], sum = 0.f;
 #pragma unroll
-        for (int s = 0; s < JOIN_PARTS; s++) o[s] = w[s] != 0.f ? p.part_o[(s * step + item) * p.hd + c] : 0.f;
+        for (int s = 0; s < JOIN_PARTS; s++) o[s] = masked_part_counts(w[s]) ? p.part_o[(s * step + item) * p.hd + c] : 0.f;
 #pragma unroll
         for (int s = 0; s < JOIN_PARTS; s++) sum = fmaf(w[s], o[s], sum);
         stf((T*)p.out + row * p.ldo + (long)h * p.hd, c, sum * inv);

@@ -346,14 +346,15 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
                     const float a0 = __shfl_sync(0xffffffffu, v[y], src), a1 = __shfl_sync(0xffffffffu, v[4 + y], src);
                     if (y == 2 * (key >> 3) + (key & 1)) w0 = a0, w1 = a1;
                 }
+                const uint32_t not_seen = __shfl_sync(0xffffffffu, unseen, src) >> (2 * (key >> 3) + (key & 1));
 #pragma unroll
                 for (int c = 0; c < DV / 8; c++)
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
                         const float e = bf16_to_f32(*reinterpret_cast<const bf16_t*>(vb + amf_at(key, 8 * c + 2 * (lane & 3) + y)));
                         if (!(fabsf(e) < INFINITY)) {
-                            if (w0 != 0.f) o[c][y] = fmaf(w0, e, o[c][y]);
-                            if (w1 != 0.f) o[c][2 + y] = fmaf(w1, e, o[c][2 + y]);
+                            if (!(not_seen & 1u)) o[c][y] = fmaf(w0, e, o[c][y]);
+                            if (!(not_seen & 16u)) o[c][2 + y] = fmaf(w1, e, o[c][2 + y]);
                         }
                     }
                 __syncwarp();
@@ -419,9 +420,9 @@ __global__ void __launch_bounds__(32 * AmfCfg<HD>::WARPS, AmfCfg<HD>::CTAS)
         float ll = 0.f, a = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) {
-            const float f = ex2_approx(ml[(w * 16 + r) * 2] - mm);
-            ll = fmaf(ml[(w * 16 + r) * 2 + 1], f, ll);
-            if (f != 0.f) a = fmaf(mo[(w * 16 + r) * DV + c], f, a);
+            const float f = ex2_approx(ml[(w * 16 + r) * 2] - mm), lw = ml[(w * 16 + r) * 2 + 1];
+            ll = fmaf(lw, f, ll);
+            if (lw != 0.f) a = fmaf(mo[(w * 16 + r) * DV + c], f, a);  // also where f has vanished: the sum may not be finite
         }
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         const long row = sq.q0 + r / p.G;

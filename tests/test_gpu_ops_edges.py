@@ -222,3 +222,25 @@ def test_parts_are_weighted_by_their_sums_under_any_bias(dtype, nh, nkv, hd, nq,
     # bias and sum in units of log 2 and back: four roundings of 2^-24
     bias = max(bias, -1e30)
     assert bool(((lse.double() - (wlse + bias)).abs() <= 2.0**-22 * abs(bias) + 2.0**-18 * wlse.abs()).all())
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("ql,kl", [([390], [390]), ([3], [390]), ([3], [5003]), ([60], [4000]), ([200], [3000])])
+def test_a_nan_counts_however_small_its_weight(dtype, nh, nkv, hd, ql, kl):
+    """Scores so far apart that nearly all weights are zero in 32 bits: a row that sees a NaN in V is still NaN, in a masked tile, a part
+    of the key axis or a warp whose weight has vanished as in any other."""
+    q, k, v = normal(47, sum(ql), nh, hd, scale=2.0, dtype=dtype), normal(48, sum(kl), nkv, hd, dtype=dtype), normal(49, sum(kl), nkv, hd, dtype=dtype)
+    n = kl[0]
+    k_doc = (torch.arange(n) % 5 == 1).to(torch.int32).cuda()
+    q_doc = torch.zeros(sum(ql), dtype=torch.int32, device="cuda")
+    opt = dict(scale=100.0, causal=True, q_doc=q_doc, k_doc=k_doc)
+    clean = attend(q, k, v, ql, kl, **opt)
+    assert bool(torch.isfinite(clean[0]).all())
+    place, _ = places(ql, kl)
+    for key in (3, n // 2 // 5 * 5, (n - 2) // 5 * 5, 6):  # the last one is hidden
+        bad = v.clone()
+        bad[key] = math.nan
+        out, lse = attend(q, k, bad, ql, kl, **opt)
+        sees = place >= key if key != 6 else torch.zeros_like(place, dtype=torch.bool)
+        assert torch.equal(lse, clean[1])
+        assert bool(torch.isnan(out[sees]).all()) and torch.equal(out[~sees], clean[0][~sees])
