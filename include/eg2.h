@@ -222,7 +222,8 @@ typedef struct {
 int64_t eg2_attention_masked_workspace(const eg2_masked_attention* args);
 int eg2_attention_masked(const eg2_masked_attention* args, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* q[r, c] = rint(x[r, c] * (127 / top)) (ties to even), scale[r] = top / 127, top = max_c |x[r, c]|. A row of zeros gets
+/* q[r, c] = rint(x[r, c] * (127 / top)) (ties to even), scale[r] = top / 127, top = max_c |x[r, c]|; q scale is within half a scale
+ * of x, the rounding of the scale apart (half of 2^-149 where top / 127 is subnormal). A row of zeros gets
  * scale 0, a row with a NaN or an infinity zeros and scale NaN. Columns [k, ldq) of q are not written. */
 int eg2_quantize_rows(int kind, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int k,
                       void* stream);

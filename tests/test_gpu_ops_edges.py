@@ -244,3 +244,29 @@ def test_a_nan_counts_however_small_its_weight(dtype, nh, nkv, hd, ql, kl):
         sees = place >= key if key != 6 else torch.zeros_like(place, dtype=torch.bool)
         assert torch.equal(lse, clean[1])
         assert bool(torch.isnan(out[sees]).all()) and torch.equal(out[~sees], clean[0][~sees])
+
+
+# ---- 8-bit integers -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("k", [1, 7, 64, 200, 777, 1000, 3000, 8192, 20_000])
+@pytest.mark.parametrize("top", [1e-30, 3.8e-37, 3.7e-37, 1e-37, 1.2e-38, 1e-38, 1e-39, 2e-40])
+def test_quantize_rows_of_the_smallest_numbers(dtype, k, top):
+    """127 / top does not fit 32 bits below 3.73e-37. The numbers are the definition's all the same: zeros stay zero, the largest is
+    127, and q * scale is within half a step of x and the rounding of the scale, half of 2^-149 where it is subnormal, 127 times."""
+    x = normal(61, 5, k).clamp(-3, 3) * (top / 4)
+    x[:, 0] = top
+    x[1] *= -1.0
+    x[2, 1:] = 0.0
+    x[3, ::2] = 0.0
+    x[4] = 0.0
+    x = x.to(dtype)
+    q, scale = ops.quantize_rows(x)
+    y = x.double()
+    most = y.abs().amax(1)
+    np.testing.assert_array_equal(scale.cpu().numpy(), most.float().cpu().numpy() / np.float32(127.0))
+    exact = y * (127.0 / most.clamp(min=1e-300))[:, None]
+    # two roundings of 2^-24 each of a number of at most 127: nothing but a tie within 127 * 2^-22 may go the other way
+    assert bool(((q.double() - exact).abs() <= 0.5 + 127 * 2.0**-22).all())
+    assert bool((q[x == 0] == 0).all()) and bool((q.long().abs().amax(1)[most > 0] == 127).all())
+    back = q.double() * scale.double()[:, None]
+    assert bool(((back - y).abs() <= scale.double()[:, None] * (0.5 + 127 * 2.0**-22) + 127 * 2.0**-150 + most[:, None] * 2.0**-24).all())
