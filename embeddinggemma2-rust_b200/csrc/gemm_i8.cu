@@ -446,6 +446,12 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
             TO* out = (TO*)p.C + (long)row0 * p.ldc + n0;
             const int rows = min(32, p.M - row0);
             auto chunk = [&](int c, uint32_t (&r)[32]) -> bool {
+                // A sum of the most columns, all -128 on both sides, is 2^31 and wraps to the one value that no other sum has; the
+                // number below it in 32 bits, 2^31 - 1, becomes 2^31 as f32.
+                if (p.K == EG2_I8_MAX_K) {
+#pragma unroll
+                    for (int q = 0; q < 32; q++) r[q] -= r[q] == 0x80000000u;
+                }
                 uint8_t* mine = stage + lane * 144 + (sizeof(TO) == 2 ? (c & 1) * 64 : 0);
 #pragma unroll
                 for (int q = 0; q < 32; q += 8) {

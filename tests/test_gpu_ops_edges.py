@@ -270,3 +270,18 @@ def test_quantize_rows_of_the_smallest_numbers(dtype, k, top):
     assert bool((q[x == 0] == 0).all()) and bool((q.long().abs().amax(1)[most > 0] == 127).all())
     back = q.double() * scale.double()[:, None]
     assert bool(((back - y).abs() <= scale.double()[:, None] * (0.5 + 127 * 2.0**-22) + 127 * 2.0**-150 + most[:, None] * 2.0**-24).all())
+
+
+@pytest.mark.parametrize("m,n", [(3, 2), (200, 70), (1800, 1600)])
+@pytest.mark.parametrize("k", [ops.I8_MAX_K, ops.I8_MAX_K - 16])
+def test_gemm_i8_sums_of_the_lowest_values(m, n, k):
+    """-128 on both sides over the most columns allowed: 2^31 itself; and the other corners of the range."""
+    a = torch.full((m, k), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((n, k), -128, dtype=torch.int8, device="cuda")
+    a[1::3], a[2::3, -1] = 127, 0
+    w[1::2] = 127
+    one = torch.ones(max(m, n), device="cuda")
+    got = ops.gemm_i8(a, one[:m], w, one[:n], out_dtype=F32)
+    rows = [(-128, k), (127, k), (-128, k - 1)]  # value and count of a row's factors
+    want = torch.tensor([[np.float32(va * c * vw) for vw in (-128, 127)] for va, c in rows]).cuda()
+    assert torch.equal(got, want[torch.arange(m) % 3][:, torch.arange(n) % 2])
