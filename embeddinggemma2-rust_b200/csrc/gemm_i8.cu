@@ -600,9 +600,10 @@ int eg2_quantize_rows(int kind, const void* x, int64_t ldx, int8_t* q, int64_t l
 
 int eg2_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw, const float* w_scale,
                 const float* bias, void* C, int64_t ldc, int64_t M, int N, int K, int out_f32, void* stream) {
-    if (M < 0 || N <= 0 || K <= 0 || K > EG2_I8_MAX_K || lda < K || ldw < K || ldc < N || lda % 16 || ldw % 16) return EG2_ERR_INVALID;
+    if (M < 0 || M > (1L << 30) || N <= 0 || N > (1 << 30) || K <= 0 || K > EG2_I8_MAX_K) return EG2_ERR_INVALID;
+    if (lda < K || ldw < K || ldc < N || lda % 16 || ldw % 16) return EG2_ERR_INVALID;
     if (M == 0) return EG2_OK;
-    if (!A || !W || !a_scale || !w_scale || !C || M > (1L << 30) || ((uintptr_t)A | (uintptr_t)W) % 16) return EG2_ERR_INVALID;
+    if (!A || !W || !a_scale || !w_scale || !C || ((uintptr_t)A | (uintptr_t)W) % 16) return EG2_ERR_INVALID;
     eg2::I8Params p{a_scale, w_scale, bias, C, ldc, (int)M, N, K, 0, 0};
     const int rc = out_f32 ? eg2::gemm_i8<float>(A, lda, W, ldw, p, (cudaStream_t)stream)
                            : eg2::gemm_i8<bf16_t>(A, lda, W, ldw, p, (cudaStream_t)stream);

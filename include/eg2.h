@@ -228,7 +228,7 @@ int eg2_attention_masked(const eg2_masked_attention* args, void* workspace, int6
 int eg2_quantize_rows(int kind, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int k,
                       void* stream);
 /* C[m, n] = (sum_k A[m, k] W[n, k]) a_scale[m] w_scale[n] + bias[n] (bias may be NULL), the sum exact in 32-bit integers.
- * C is f32 when out_f32 != 0, else bf16. Any M, N and K; A and W 16-byte aligned, lda and ldw multiples of 16. */
+ * C is f32 when out_f32 != 0, else bf16. M and N up to 2^30; A and W 16-byte aligned, lda and ldw multiples of 16. */
 #define EG2_I8_MAX_K 131072 /* sums of any int8 values are exact: from -128 * 127 * K to 128 * 128 * K = 2^31 */
 int eg2_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw, const float* w_scale,
                 const float* bias, void* C, int64_t ldc, int64_t M, int N, int K, int out_f32, void* stream);
