@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
     if (t == 0) scale[row] = qr.scale;
 }
 
-// Longer rows: a block per row, two passes over it (the second from L2).
+// Longer rows: a block per row, two passes over it (the second from L2). Columns are unsigned: k may be 2^31 - 1, and c ends above it.
 template <typename T>
 __global__ void __launch_bounds__(512) quantize_rows_long_kernel(const T* __restrict__ x, long ldx, int8_t* __restrict__ q,
                                                                  long ldq, float* __restrict__ scale, int k) {
@@ -199,13 +199,13 @@ __global__ void __launch_bounds__(512) quantize_rows_long_kernel(const T* __rest
     const T* xr = x + row * ldx;
     uint32_t top = 0;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < k; c += 512) top = max(top, quant_bits(ldf(xr, c)));
+    for (unsigned c = threadIdx.x; c < (unsigned)k; c += 512) top = max(top, quant_bits(ldf(xr, c)));
     const QuantRow qr = quant_row(quant_max<512>(top, slot));
     if (qr.tiny) {
-        for (int c = threadIdx.x; c < k; c += 512) q[row * ldq + c] = (int8_t)(quant_one(ldf(xr, c) * QUANT_UP, qr.inv) & 0xff);
+        for (unsigned c = threadIdx.x; c < (unsigned)k; c += 512) q[row * ldq + c] = (int8_t)(quant_one(ldf(xr, c) * QUANT_UP, qr.inv) & 0xff);
     } else {
 #pragma unroll 4
-        for (int c = threadIdx.x; c < k; c += 512) q[row * ldq + c] = qr.bad ? (int8_t)0 : (int8_t)(quant_one(ldf(xr, c), qr.inv) & 0xff);
+        for (unsigned c = threadIdx.x; c < (unsigned)k; c += 512) q[row * ldq + c] = qr.bad ? (int8_t)0 : (int8_t)(quant_one(ldf(xr, c), qr.inv) & 0xff);
     }
     if (threadIdx.x == 0) scale[row] = qr.scale;
 }

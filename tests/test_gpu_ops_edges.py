@@ -272,6 +272,16 @@ def test_quantize_rows_of_the_smallest_numbers(dtype, k, top):
     assert bool(((back - y).abs() <= scale.double()[:, None] * (0.5 + 127 * 2.0**-22) + 127 * 2.0**-150 + most[:, None] * 2.0**-24).all())
 
 
+def test_quantize_rows_of_a_row_of_the_most_columns():
+    k = 2**31 - 1
+    x = torch.zeros(1, k, dtype=BF16, device="cuda")
+    x[0, 0], x[0, -1], x[0, -400], x[0, k // 2] = 2.0, -4.0, 1.0, 3.0
+    q, scale = ops.quantize_rows(x)
+    assert float(scale[0]) == float(np.float32(4.0) / np.float32(127.0))
+    assert [int(q[0, c]) for c in (0, k - 1, k - 400, k // 2)] == [64, -127, 32, 95]  # 63.5 to even, 31.75, 95.25
+    assert int((q != 0).sum()) == 4
+
+
 @pytest.mark.parametrize("m,n", [(3, 2), (200, 70), (1800, 1600)])
 @pytest.mark.parametrize("k", [ops.I8_MAX_K, ops.I8_MAX_K - 16])
 def test_gemm_i8_sums_of_the_lowest_values(m, n, k):
