@@ -255,7 +255,8 @@ int eg2_rotary(int kind, int layout, int inverse, const void* q, int64_t ldq, in
     if (layout != EG2_ROTARY_HALF && layout != EG2_ROTARY_INTERLEAVED) return EG2_ERR_INVALID;
     if (rows < 0 || nh < 0 || nkv < 0 || nh + nkv <= 0 || hd <= 0 || rot_dim <= 0 || rot_dim > hd || rot_dim % 2)
         return EG2_ERR_INVALID;
-    if ((long)nh * hd > 0x7fffffffL || (long)nkv * hd > 0x7fffffffL || rows > (1L << 40) / hd) return EG2_ERR_INVALID;
+    // A channel's number and a few units of 16 bytes stay below 2^31.
+    if (hd > (1 << 30) || (long)nh * hd > 0x7fffffffL || (long)nkv * hd > 0x7fffffffL || rows > (1L << 40) / hd) return EG2_ERR_INVALID;
     if (nh && (!q || !q_out || ldq < (long)nh * hd || ldqo < (long)nh * hd)) return EG2_ERR_INVALID;
     if (nkv && (!k || !k_out || ldk < (long)nkv * hd || ldko < (long)nkv * hd)) return EG2_ERR_INVALID;
     if (rows == 0) return EG2_OK;

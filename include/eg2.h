@@ -179,7 +179,7 @@ enum { EG2_SCALING_NONE = 0, EG2_SCALING_LINEAR = 1, EG2_SCALING_NTK = 2, EG2_SC
 int eg2_rotary_steps(int rot_dim, double theta, int scaling, double factor, double original_len, uint64_t* steps,
                      float* magnitude);
 
-/* q [rows, nh, hd] and k [rows, nkv, hd] (either count may be 0) with row strides ldq / ldk into q_out / k_out, which may
+/* q [rows, nh, hd] and k [rows, nkv, hd] (either count may be 0, hd up to 2^30) with row strides ldq / ldk into q_out / k_out, which may
  * be the inputs themselves (same stride) but not overlap them otherwise. pos [rows], any int32; steps as above, on the
  * device. inverse != 0 turns back by the same angles (the gradient of the forward form), times magnitude all the same. */
 int eg2_rotary(int kind, int layout, int inverse, const void* q, int64_t ldq, int nh, const void* k, int64_t ldk, int nkv,
