@@ -201,9 +201,13 @@ def attention_masked(q, k, v, q_off, k_off, max_q: int, max_k: int, *, scale: fl
     def ptr(t):
         return 0 if t is None else t.data_ptr()
 
-    a = _MASKED.pack(KINDS[kind], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(lse), ldq, ldk, ldv, ldo,
-                     q_off.data_ptr(), k_off.data_ptr(), q_rows, k_rows, n_seq, int(max_q), int(max_k), nh, nkv, hd, scale, softcap,
-                     int(window), 1 if causal else 0, ptr(prefix_len), ptr(q_doc), ptr(k_doc), ptr(slopes), ptr(dist_bias), radius)
+    try:
+        a = _MASKED.pack(KINDS[kind], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(lse), ldq, ldk, ldv, ldo,
+                         q_off.data_ptr(), k_off.data_ptr(), q_rows, k_rows, n_seq, int(max_q), int(max_k), nh, nkv, hd, scale, softcap,
+                         int(window), 1 if causal else 0, ptr(prefix_len), ptr(q_doc), ptr(k_doc), ptr(slopes), ptr(dist_bias), radius)
+    except (struct.error, OverflowError) as e:
+        _bad(f"attention_masked: a number does not fit 32 bits (max_q {max_q}, max_k {max_k}, window {window}, scale {scale}, "
+             f"softcap {softcap}): {e}")
     lib = L.load()
     need = lib.eg2_attention_masked_workspace(a)
     if need < 0:

@@ -295,3 +295,14 @@ def test_gemm_i8_sums_of_the_lowest_values(m, n, k):
     rows = [(-128, k), (127, k), (-128, k - 1)]  # value and count of a row's factors
     want = torch.tensor([[np.float32(va * c * vw) for vw in (-128, 127)] for va, c in rows]).cuda()
     assert torch.equal(got, want[torch.arange(m) % 3][:, torch.arange(n) % 2])
+
+
+# ---- numbers that do not fit the C call ----------------------------------------------------------------------
+@pytest.mark.parametrize("change", [dict(window=2**31), dict(window=-(2**40)), dict(scale=1e39), dict(softcap=1e300), dict(softcap=math.nan),
+                                    dict(max_q=2**31), dict(max_k=2**40), dict(max_q=-1)])
+def test_attention_refuses_numbers_that_do_not_fit(change):
+    q = normal(71, 4, 2, 64, dtype=BF16)
+    a = dict(max_q=4, max_k=4)
+    a.update(change)
+    with pytest.raises(L.Eg2Error):
+        ops.attention_masked(q, q, q, offsets([4]), offsets([4]), a.pop("max_q"), a.pop("max_k"), **a)
