@@ -27,6 +27,7 @@ KINDS = {torch.bfloat16: L.EG2_BF16, torch.float32: L.EG2_F32}
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 I8_MAX_K = 131072
+_INT = 2**31 - 1  # what the C call's int holds
 
 
 def _bad(msg: str):
@@ -63,6 +64,8 @@ def _heads(t, name: str, kind=None):
     if t.dim() != 3 or t.dtype not in KINDS or (kind is not None and t.dtype != kind):
         _bad(f"{name}: expected a [rows, heads, channels] tensor of {kind or 'bf16 or f32'}, got {tuple(t.shape)} {t.dtype}")
     rows, heads, hd = t.shape
+    if heads * hd > _INT:
+        _bad(f"{name}: {heads} heads of {hd} channels are 2^31 or more")
     row, head, ch = t.stride()
     if ch == 1 and head == hd and row >= heads * hd:
         return row
@@ -89,6 +92,8 @@ def rotary_steps(rot_dim: int, theta: float = 10000.0, scaling: str = "none", fa
     is the device array that :func:`rotary` takes."""
     if scaling not in SCALINGS:
         _bad(f"unknown scaling {scaling!r}: one of {', '.join(SCALINGS)}")
+    if int(rot_dim) > _INT:
+        _bad(f"rot_dim {rot_dim} is 2^31 or more")
     steps = np.zeros(max(1, int(rot_dim) // 2), np.uint64)
     m = C.c_float()
     _check(L.load().eg2_rotary_steps(int(rot_dim), float(theta), SCALINGS[scaling], float(factor), float(original_len),
@@ -226,8 +231,8 @@ def quantize_rows(x):
     if x.dim() != 2 or x.dtype not in KINDS or (x.shape[1] > 1 and x.stride(1) != 1):
         _bad(f"x: expected [rows, k] of bf16 or f32 with contiguous rows, got {tuple(x.shape)} {x.dtype}")
     rows, k = x.shape
-    if k == 0:
-        _bad("x has no columns")
+    if k == 0 or k > _INT:
+        _bad(f"x has {k} columns: none, or 2^31 or more")
     ldx = x.stride(0) if rows > 1 else max(x.stride(0), k)
     if ldx < k:
         _bad(f"x: the rows overlap (strides {x.stride()})")
@@ -258,6 +263,8 @@ def gemm_i8(a, a_scale, w, w_scale, *, bias=None, out_dtype=torch.bfloat16, out=
     (m, k), n = a.shape, w.shape[0]
     if w.shape[1] != k or k == 0 or k > I8_MAX_K:
         _bad(f"a {tuple(a.shape)} and w {tuple(w.shape)} do not match, or more than {I8_MAX_K} columns")
+    if n > _INT:
+        _bad(f"w has {n} rows, 2^31 or more")
     _floats(a_scale, "a_scale", m)
     _floats(w_scale, "w_scale", n)
     if out is None:
