@@ -306,3 +306,38 @@ def test_attention_refuses_numbers_that_do_not_fit(change):
     a.update(change)
     with pytest.raises(L.Eg2Error):
         ops.attention_masked(q, q, q, offsets([4]), offsets([4]), a.pop("max_q"), a.pop("max_k"), **a)
+
+
+# ---- graphs ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nq", [700, 2])
+def test_the_calls_can_be_captured_in_a_graph(nq):
+    """All of them in one graph, the attention's workspace among them (few queries split the key axis); replayed on other
+    inputs it gives what the calls give."""
+    nh, nkv, hd, nk = 4, 2, 128, 3000
+    x = normal(81, nk, 512, dtype=BF16)
+    w, ws = ops.quantize_rows(normal(82, (nh + 2 * nkv) * hd, 512, scale=512**-0.5))
+    steps = torch.from_numpy(ops.rotary_steps(hd)[0].view(np.int64)).cuda()
+    pos = torch.arange(nk, dtype=torch.int32).cuda()
+    q_off, k_off = offsets([nq]), offsets([nk])
+
+    def layer():
+        qkv = ops.gemm_i8(*ops.quantize_rows(x), w, ws)
+        q, k, v = (t.unflatten(1, (-1, hd)) for t in qkv.split([nh * hd, nkv * hd, nkv * hd], 1))
+        q, k = ops.rotary(q, k, pos, steps)
+        return ops.attention_masked(q[nk - nq :], k, v, q_off, k_off, nq, nk, scale=hd**-0.5, softcap=30.0, causal=True, return_lse=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer()
+    for seed in (83, 84):
+        x.copy_(normal(seed, nk, 512, dtype=BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = layer()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert L.load().eg2_device_status() == 0
