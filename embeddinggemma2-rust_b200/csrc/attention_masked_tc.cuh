@@ -35,7 +35,8 @@
 // twice over the tiles that held such elements, with 1 for each of them in V and 1 for each visible key in P: where this
 // product is positive the row sees an infinity of that sign, or a NaN, in that channel, and takes it. So no visible bit
 // depends on what hidden keys hold, at no cost while all is finite; where it is not, a unit's time grows by its one
-// repetition and the tiles concerned, whatever their number, never by rows taken one by one.
+// repetition and the tiles concerned, whatever their number, never by rows taken one by one (8,192 tokens, 8 heads over 2 of 128: causal 139 us, with
+// one NaN 728, with NaN alone 3,011; with 40 NaN rows of a hidden document 322 and 1,140).
 
 constexpr int AMT_THREADS = 384;
 constexpr int AMT_MASK_WORDS = EG2_MASKED_MAX_LEN / 128 / 32;
@@ -184,40 +185,63 @@ struct TileWalk {
 };
 
 // Prepares one 16 KB chunk of a V tile (128 keys of 128 bytes, whatever the order of the 16-byte units in a row) for the
-// unit's stage; rows from `live` on become zero. Whether some other element was not finite.
+// unit's stage; rows from `live` on become zero. Whether some other element was not finite, in the whole warp. Looks before it writes:
+// most chunks have none, and loads alone are under way together.
 EG2_DEV bool guard_chunk(uint8_t* chunk, int live, int stage) {
     const int lane = threadIdx.x & 31;
+    uint4* const units = reinterpret_cast<uint4*>(chunk);
+    // Top bits of the halves whose exponent is full.
+    auto odd_halves = [](uint32_t w) -> uint32_t { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+    const int end = 8 * max(min(live, 128), 0);
     bool hit = false;
-    for (int x = lane; x < 1024; x += 32) {
-        uint4* at = reinterpret_cast<uint4*>(chunk) + x;
-        if ((x >> 3) >= live) {
-            *at = make_uint4(0u, 0u, 0u, 0u);
-        } else if (stage) {
-            const uint4 v = *at;
+    if (stage) {
+        uint32_t odd = 0u;
+#pragma unroll 4
+        for (int x = lane; x < 1024; x += 32) {
+            const uint4 v = units[x];
+            const uint32_t o = odd_halves(v.x) | odd_halves(v.y) | odd_halves(v.z) | odd_halves(v.w);
+            odd |= x < end ? o : 0u;
+        }
+        hit = __any_sync(0xffffffffu, odd != 0u);
+    }
+    if (hit || stage > 1) {
+#pragma unroll 1
+        for (int x = lane; x < end; x += 32) {
+            const uint4 v = units[x];
             uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            // Past stage 1 an infinity of the other sign is not meant.
+            const uint32_t other = stage == 2 ? 0xff80u : 0x7f80u;
 #pragma unroll
             for (int y = 0; y < 4; y++) {
-                uint32_t r = 0u;
-#pragma unroll
-                for (int z = 0; z < 32; z += 16) {
-                    const uint32_t e = (w[y] >> z) & 0xffffu;
-                    const bool odd = (e & 0x7f80u) == 0x7f80u, takes = e != (stage == 2 ? 0xff80u : 0x7f80u);  // NaN, or the sign asked for
-                    hit |= odd;
-                    r |= (stage == 1 ? (odd ? 0u : e) : odd && takes ? 0x3f80u : 0u) << z;
-                }
-                w[y] = r;
+                uint32_t odd = odd_halves(w[y]);
+                if (stage > 1) odd &= ((w[y] & 0xffffu) == other ? 0u : 0x8000u) | ((w[y] >> 16) == other ? 0u : 0x80000000u);
+                const uint32_t ones = odd >> 15;  // 1 in each half that counts
+                w[y] = stage == 1 ? w[y] & ~(ones * 0xffffu) : ones * 0x3f80u;
             }
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
+            units[x] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
+    for (int x = end + lane; x < 1024; x += 32) units[x] = make_uint4(0u, 0u, 0u, 0u);
     return hit;
+}
+
+// The columns of a tile that the staged table hides; a call, since it is rare and the loop over scores is faster without its code.
+__device__ __noinline__ uint4 masked_hidden_columns(const float* table) {
+    uint4 h = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+    for (int c = 0; c < 32; c++) {
+        if (table[c] == -INFINITY) h.x |= 1u << c;
+        if (table[32 + c] == -INFINITY) h.y |= 1u << c;
+        if (table[64 + c] == -INFINITY) h.z |= 1u << c;
+        if (table[96 + c] == -INFINITY) h.w |= 1u << c;
+    }
+    return h;
 }
 
 // A softmax warp's part of a unit in stages 2 and 3: weights of 1 for the visible keys of its group's tiles, then, where the
 // product is positive, the infinity to the sums that stage 1 wrote (of both signs, or with a NaN, they make NaN). False where a
-// wait ran out. Apart from the loop over scores, whose speed goes by what else is compiled into it (8,192 tokens without a mask, 8 heads
-// over 2 of 128: 288 us, 372 with these weights as a branch inside that loop).
-template <int HD>
+// wait ran out.
+template <int HD, bool TABLES>
 EG2_DEV bool masked_count_unit(const AmtParams& ap, const AmtUnit& u, uint32_t tmem, int T, int U, uint64_t* s_full, uint64_t* p_full,
                                uint64_t* pv_done, uint64_t* o_empty, uint64_t* e_bar, volatile int* abort_flag) {
     using Cfg = AmtCfg<HD>;
@@ -245,10 +269,10 @@ EG2_DEV bool masked_count_unit(const AmtParams& ap, const AmtUnit& u, uint32_t t
         for (int x = 0; x < 128; x += 32) {
             const int a = min(max(lo - kbase - x, 0), 32), z = min(max(hi - kbase - x, 0), 32);
             uint32_t seen = z > a ? (0xffffffffu >> (32 - z)) & (0xffffffffu << a) : 0u, pk[16];
-            if (docs || p.table)
+            if (docs || (TABLES && p.table))
                 for (uint32_t left = seen; left; left &= left - 1u) {
                     const int key = kbase + x + __ffs(left) - 1;
-                    if ((docs && p.k_doc[u.sq.k0 + key] != qdoc) || (p.table && masked_table(p, head, key - place) == -INFINITY))
+                    if ((docs && p.k_doc[u.sq.k0 + key] != qdoc) || (TABLES && p.table && masked_table(p, head, key - place) == -INFINITY))
                         seen &= ~(left & (~left + 1u));
                 }
             __syncwarp();
@@ -294,6 +318,23 @@ EG2_DEV bool masked_count_unit(const AmtParams& ap, const AmtUnit& u, uint32_t t
     __syncwarp();
     mbar_arrive_if(o_empty, lane == 0);
     return true;
+}
+
+// The same as a call or as code of the kernel: the loop over scores does not use it, but its speed goes by what else is compiled into the
+// kernel. 8,192 tokens, as a call / inlined (12 heads of 64, 8 over 2 of 128, 4 over 2 of 256): plain 420 / 389, 352 / 291 and 285 / 293 us,
+// a table 561 / 594, 442 / 498 and 377 / 348, capped 633 / 655, 483 / 483 and 348 / 367. As a branch inside the loop 372 at head 128, plain.
+template <int HD, bool TABLES>
+__device__ __noinline__ bool masked_count_call(const AmtParams& ap, const AmtUnit& u, uint32_t tmem, int T, int U, uint64_t* s_full,
+                                               uint64_t* p_full, uint64_t* pv_done, uint64_t* o_empty, uint64_t* e_bar, volatile int* abort_flag) {
+    return masked_count_unit<HD, TABLES>(ap, u, tmem, T, U, s_full, p_full, pv_done, o_empty, e_bar, abort_flag);
+}
+template <int HD, bool TABLES>
+EG2_DEV bool masked_count(const AmtParams& ap, const AmtUnit& u, uint32_t tmem, int T, int U, uint64_t* s_full, uint64_t* p_full,
+                          uint64_t* pv_done, uint64_t* o_empty, uint64_t* e_bar, volatile int* abort_flag) {
+    if constexpr (HD == 512 || (HD <= 128 && !TABLES))
+        return masked_count_unit<HD, TABLES>(ap, u, tmem, T, U, s_full, p_full, pv_done, o_empty, e_bar, abort_flag);
+    else
+        return masked_count_call<HD, TABLES>(ap, u, tmem, T, U, s_full, p_full, pv_done, o_empty, e_bar, abort_flag);
 }
 
 // The score's parts that a kernel is compiled for; AMT_ANY decides at run time. The softmax is long straight code, and what
@@ -577,7 +618,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                             bool hit = false;
                             for (int c = 0; c < Cfg::UCH; c++)
                                 hit |= guard_chunk(smem + Cfg::OFF_V + u * Cfg::UNIT + c * 16384, un->sq.nk - kt * 128, un->stage);
-                            if (un->stage == 1 && __any_sync(0xffffffffu, hit) && lane == 0) {
+                            if (un->stage == 1 && hit && lane == 0) {
                                 un->bad[kt >> 5] |= 1u << (kt & 31);
                                 un->found = 1;
                             }
@@ -829,7 +870,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
             if (!un) break;
             const int n = un->n;
             if (un->stage >= 2) {
-                if (!(ok = masked_count_unit<HD>(ap, *un, tmem, T, U, s_full, p_full, pv_done, o_empty, e_bar, abort_flag))) break;
+                if (!(ok = masked_count<HD, (PARTS & (AMT_TAB | AMT_ANY)) != 0>(ap, *un, tmem, T, U, s_full, p_full, pv_done, o_empty, e_bar, abort_flag))) break;
                 T += n;
                 U++;
                 if (lane == 0) mbar_arrive(&unit_empty[i & 1]);
@@ -892,31 +933,33 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
                     const uint32_t ts = tmem + 128 * buf + lane_off;
                     const bool sees = kbase < some_hi && kbase + NC > some_lo;
                     const bool docs = p.q_doc && ((un->docs[kbase >> 12] >> ((kbase >> 7) & 31)) & 1u);
-                    const bool full = !docs && !(tables && hides) && kbase >= all_lo && kbase + NC <= all_hi;
+                    const bool some = docs || (tables && hides);
+                    const bool full = !some && kbase >= all_lo && kbase + NC <= all_hi;
                     any_masked |= !full;
                     uint32_t same[4] = {~0u, ~0u, ~0u, ~0u};  // columns of this row's document that no bias hides
-                    if (docs && sees) {
-                        // The rows of a warp are of few documents, mostly one: a ballot per document and 32 columns.
-                        uint32_t left = __ballot_sync(0xffffffffu, lo < hi);
+                    if (some && sees) {
+                        if (docs) {
+                            // The rows of a warp are of few documents, mostly one: a ballot per document and 32 columns.
+                            uint32_t left = __ballot_sync(0xffffffffu, lo < hi);
 #pragma unroll
-                        for (int x = 0; x < 4; x++) same[x] = 0u;
-                        while (left) {
-                            const int d = __shfl_sync(0xffffffffu, qdoc, __ffs(left) - 1);
-                            left &= ~__ballot_sync(0xffffffffu, qdoc == d);
+                            for (int x = 0; x < 4; x++) same[x] = 0u;
+                            while (left) {
+                                const int d = __shfl_sync(0xffffffffu, qdoc, __ffs(left) - 1);
+                                left &= ~__ballot_sync(0xffffffffu, qdoc == d);
 #pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                const uint32_t cols = __ballot_sync(0xffffffffu, ids[x] == d);
-                                if (qdoc == d) same[x] = cols;
+                                for (int x = 0; x < 4; x++) {
+                                    const uint32_t cols = __ballot_sync(0xffffffffu, ids[x] == d);
+                                    if (qdoc == d) same[x] = cols;
+                                }
                             }
                         }
-                    }
-                    if (tables && hides && sees) {
-                        const float* tb = my_table + min(max(kbase - place, -p.radius - 128), p.radius) + p.radius + 128;
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-#pragma unroll 1
-                            for (int c = 0; c < 32; c++)
-                                if (tb[32 * x + c] == -INFINITY) same[x] &= ~(1u << c);
+                        if (tables && hides) {
+                            const uint4 h = masked_hidden_columns(my_table + min(max(kbase - place, -p.radius - 128), p.radius) + p.radius + 128);
+                            same[0] &= ~h.x;
+                            same[1] &= ~h.y;
+                            same[2] &= ~h.z;
+                            same[3] &= ~h.w;
+                        }
                     }
                     if (j + 2 < n) {
                         walk.next();
