@@ -524,9 +524,9 @@ static int attention_masked_join(const MaskedParams& p, cudaStream_t s) {
 // How a call runs. The tensor cores take bf16 whose rows and heads TMA can address (16-byte multiples) and G query
 // heads that divide a 128-row tile are packed into it, unless their bias tables together pass the shared memory
 // kept for them; the rest runs on the CUDA cores. Calls whose query tiles would be at most an eighth full -- 16 rows --
-// are bound by reading K and V and take the form made for that (4 heads over 2 of 256, up to 8 x 11,774 keys: 1 query each 43 us,
-// 60 in 128-row tiles, 8 queries each 55 and 63; 64 x 512 keys, 12 heads of 64: 47 and 71; only at a few hundred keys and all 16
-// rows do the tiles win: 8 queries over 300, 22 and 19). Packing: 256 sequences of 17 tokens, 4 heads over 1 of 256, 24 us, 64
+// are bound by reading K and V and take the form made for that (4 heads over 2 of 256, 8 x up to 11,774 keys: 1 query each 42 us,
+// 75 in 128-row tiles, both with L2 flushed and one call at a time (33 among other calls); 8 queries each 54 and 77; 64 x 512 keys, 12 heads
+// of 64: 53 and 57; only at a few hundred keys and all 16 rows do the tiles win: 8 queries over 300, 28 and 21). Packing: 256 sequences of 17 tokens, 4 heads over 1 of 256, 24 us, 64
 // with a tile per head.
 struct MaskedPlan {
     bool tc, few;

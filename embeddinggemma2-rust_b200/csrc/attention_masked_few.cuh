@@ -2,9 +2,9 @@
 //
 // At most 16 rows (query tokens x the G heads of a K/V head): the work is to read K and V once, so the design is for
 // bytes in flight and a short path per byte, not for tensor throughput -- warp-level mma.sync with the 16 rows as M.
-// (One token of 4 heads over 2 of 256 for each of 8 documents of up to 11,774 cached keys: 33 us, 3.4 TB/s; 4 queries each over
-// 11,774 keys, 4 heads over 1 of 128: 25 us, 27 in the 128-row tiles of the tcgen05 form, whose first tiles wait for their
-// instructions.)
+// (One token of 4 heads over 2 of 256 for each of 8 documents of up to 11,774 cached keys: 33 us, 3.4 TB/s; 4 queries over
+// 30,000 keys, 4 heads over 2 of 128, a window of 20,000: 26 us, 30 in the 128-row tiles of the tcgen05 form, whose first tiles wait for
+// their instructions.)
 //
 // A CTA takes one part of the keys of one (sequence, K/V head, 256-channel half of O); each of its warps walks blocks
 // of 16 keys on its own, with a ring of its own that one lane fills by TMA, 16 keys x 64 channels a box, and its own

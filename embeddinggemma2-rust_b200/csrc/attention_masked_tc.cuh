@@ -20,12 +20,14 @@
 //               that need the document ids row by row, from the ranges of ids in the tile
 //   warps 4-11  softmax and the O / l epilogue
 //
-// Bound by issuing the softmax: 12,001 tokens under a causal mask with a prefix, capped, with slopes, 8 heads over 2 of 128:
-// 615 us; 8,192 tokens without a mask 279 us, 984 TFLOP/s.
+// Bound by the latency of the softmax at heads 64 and 128 (two warps a scheduler, which issue in 43 % of the cycles and wait for fixed
+// latencies, TMEM and instructions in the rest; no pipe is past 55 %), by products and their loads at 256 and 512, whose rings hold two
+// units and less than a tile: 12,001 tokens under a causal mask with a prefix, capped, with slopes, 8 heads over 2 of 128: 622 us; 8,192
+// tokens without a mask 290 us, 948 TFLOP/s.
 //
 // The score of a pair lives in the log2 domain (scale, cap and biases carry log2 e), so a weight is one FMA and
 // one ex2. O is rescaled only when a row's maximum grows by more than 2^8: a stale maximum is exact. l sums the
-// weights in f32 as they are, P rounds them to bf16: the product with V takes 16-bit operands, and 2^-9 of a weight
+// weights in f32 as they are, P rounds them to bf16: the product with V takes 16-bit operands, and 2^-8 of a weight
 // is what the 16-bit result carries anyway.
 //
 // Hidden keys are masked by selection, so what K holds there is harmless, but a NaN or infinity in a hidden V row
@@ -339,8 +341,8 @@ EG2_DEV bool masked_count(const AmtParams& ap, const AmtUnit& u, uint32_t tmem, 
 
 // The score's parts that a kernel is compiled for; AMT_ANY decides at run time. The softmax is long straight code, and what
 // a call does not need costs it instruction fetches. 8,192 tokens, 12 heads of 64 / 8 over 2 of 128 / 4 over 2
-// of 256, decided at run time and compiled for the call: plain 427 / 323 / 289 and 432 / 279 / 269 us, capped 742 / 523 / 375 and 657 / 474 / 345, slopes
-// 593 / 447 / 338 and 545 / 386 / 300, a table 701 / 546 / 349 and 584 / 411 / 319. `raw` below stays a test at run time in
+// of 256, decided at run time and compiled for the call: plain 471 / 373 / 301 and 393 / 295 / 287 us, capped 743 / 543 / 381 and 655 / 489 / 352, slopes
+// 619 / 455 / 358 and 526 / 414 / 328, a table 652 / 496 / 395 and 571 / 432 / 345. `raw` below stays a test at run time in
 // each: with it known, the compiler mixes the parts with the mask's code and spills (table 588 / 560 / 378 us).
 constexpr int AMT_CAP = 1, AMT_SLOPES = 2, AMT_TAB = 4, AMT_ANY = 8;
 
@@ -857,7 +859,10 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const float a = capped ? p.scale / p.softcap : p.scale * AMT_LOG2E;
         const bool raw = !(p.softcap > 0.f) && !p.slopes && !p.table && a > 0.f;
         const float sc = raw ? a : 1.f;
-        // cap2 tanh(a s) = s (c0 + c1 s^2 + ...) where |a s| <= 1/2, as long as the powers of a stay in range.
+        // cap2 tanh(a s) = s (c0 + c1 s^2 + ...) where |a s| <= 1/2, as long as the powers of a stay in range: of scale / softcap between
+        // 1e-4 and 1e3, and |score| <= softcap / 2. A warp's tile with a score past that is done twice, and so is every tile outside
+        // that range of a: 8,192 tokens, scores of deviation 2 under a cap of 50 / of 5: 655 / 1,300 us (12 heads of 64), 485 / 900 (8 over 2
+        // of 128), 352 / 560 (4 over 2 of 256), 1,062 / 1,478 (4 over 1 of 512).
         const bool near_ok = fabsf(a) > 1e-4f && fabsf(a) < 1e3f;
         const float near_max = near_ok ? (AMT_TANH_MAX / a) * (AMT_TANH_MAX / a) : -1.f;
         const float c0 = AMT_T0 * a * cap2, c1 = AMT_T1 * a * a * a * cap2, c2 = AMT_T2 * (a * a) * (a * a) * a * cap2,

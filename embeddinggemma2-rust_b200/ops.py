@@ -7,6 +7,7 @@ prefix masks, weights held in 8 bits. Each call launches the library's kernels o
 its tensors' device and returns without waiting; results are new tensors unless ``out`` is given. A tensor of
 the wrong type, shape, stride or device, and what the library refuses, raises :class:`lib.Eg2Error`.
 
+Results carry no gradient history, whatever ``requires_grad`` of the inputs says; outputs must not overlap inputs, except where it is said.
 A bounded device wait that ran out is not raised by the call: after synchronising, ``eg2_device_status`` tells.
 A tensor that is used on another stream than the one it was made on is kept alive and ordered by the caller,
 as for any torch operation.
@@ -157,8 +158,9 @@ def attention_masked(q, k, v, q_off, k_off, max_q: int, max_k: int, *, scale: fl
     Scores: ``scale * q.k``, capped to ``softcap * tanh(. / softcap)``, minus ``slopes[h] * |j - i|``, plus
     ``dist_bias[h, clamp(j - i, -R, R) + R]`` (``[nh, 2 R + 1]``). Query ``i`` sees key ``j`` within ``window`` places
     (< 0: any), with ``causal`` only ``j <= i`` or ``j < prefix_len[b]``, and only where ``q_doc`` and ``k_doc`` (int32 per
-    row) agree. A query that sees nothing gets zeros (log-sum -inf). Returns ``out`` like ``q``, with ``return_lse``
-    also the log-sums ``[q_rows, nh]``."""
+    row) agree, and not where its bias is -inf. A query that sees nothing gets zeros (log-sum -inf). Returns ``out`` like
+    ``q``, with ``return_lse`` also the log-sums ``[q_rows, nh]``; rows of no sequence, or past ``max_q`` in theirs, are left as they
+    are in memory."""
     kind = q.dtype
     ldq, ldk, ldv = _heads(q, "q"), _heads(k, "k", kind), _heads(v, "v", kind)
     q_rows, nh, hd = q.shape

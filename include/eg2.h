@@ -157,12 +157,13 @@ int eg2_attention_noalloc(const void* q, const void* k, const void* v, void* out
                           int nh, int nkv, int hd, int window, void* stream);
 
 /* ---- operators of one encoder layer in other forms than the two towers use ----------------------
- * No counterpart in the reference. All three take device pointers, allocate nothing, copy nothing, run
+ * No counterpart in the reference. All take device pointers, allocate nothing, copy nothing, run
  * asynchronously on `stream` (NULL: the default stream) and check what the host can see before they launch
  * (EG2_ERR_INVALID, nothing written). A bounded device wait that ran out is not returned: synchronise the stream, then
  * read eg2_device_status() (non-zero: results since then are not valid). kind: EG2_BF16 or EG2_F32, the type of the activations; arithmetic,
- * sums and softmax statistics are f32. Row strides are in elements; the channels of a head and the heads of
- * a row are contiguous. */
+ * sums and softmax statistics are f32, the attention's weights bf16 in its product with V where the activations are (f32
+ * else). Row strides are in elements; the channels of a head and the heads of a row are contiguous. Outputs must not overlap inputs,
+ * except where it is said. */
 
 /* Rotary positions. A pair (a, b) of channels at position p becomes
  * m (a cos t - b sin t, b cos t + a sin t), t = p f. Pair i of the rotated `rot_dim` channels is (i, i + rot_dim / 2)
@@ -194,15 +195,16 @@ int eg2_rotary(int kind, int layout, int inverse, const void* q, int64_t ldq, in
  * i and j are places among its keys, its queries being the last places. Query i sees key j when |j - i| <= window
  * (window < 0: any distance), and with causal j <= i or j < prefix_len[b], and with documents q_doc[row of i] ==
  * k_doc[row of j]. Finite entries of dist_bias below -1e30 count as -1e30 (a row that sees nothing else keeps its
- * softmax), -infinity hides. A query that sees no key gets out 0 and lse -inf; what hidden keys hold (NaN, infinities) does not
- * reach any row. A row that sees a NaN, or an infinite value, ends NaN or infinite.
+ * softmax), -infinity is a mask. A query that sees no key gets out 0 and lse -inf; what hidden keys hold (NaN, infinities) does not
+ * change a bit of any row. A row that sees a NaN, or an infinite value, ends NaN or infinite, however small the key's weight: a
+ * channel of V with infinities of one sign in that infinity (or NaN, where the weight has vanished in f32).
  * hd up to 512. bf16 runs on the tensor cores when hd, the strides and the pointers are multiples of 8 elements. */
 #define EG2_MASKED_MAX_LEN (1 << 20) /* tokens of one sequence */
 #define EG2_MASKED_MAX_RADIUS 1024
 typedef struct {
     int kind;
     const void *q, *k, *v; /* [q_rows, nh, hd], [k_rows, nkv, hd] */
-    void* out;             /* [q_rows, nh, hd]; rows of no sequence are not written */
+    void* out;             /* [q_rows, nh, hd]; rows of no sequence, or past max_q in theirs, are not written, nor in lse */
     float* lse;            /* [q_rows, nh] or NULL */
     int64_t ldq, ldk, ldv, ldo;
     const int32_t *q_off, *k_off; /* [n_seq + 1] */
