@@ -606,6 +606,11 @@ int eg2_attention_masked(const eg2_masked_attention* a, void* workspace, int64_t
     MaskedParams p{a->q, a->k, a->v, a->out, a->lse, a->ldq, a->ldk, a->ldv, a->ldo, a->q_off, a->k_off, a->prefix_len, a->q_doc,
                    a->k_doc, a->slopes, a->dist_bias, a->q_rows, a->k_rows, a->n_seq, a->max_q, a->max_k, a->nh, a->nkv, a->hd,
                    a->nh / a->nkv, a->window, a->causal, a->dist_radius, 1, 0, a->scale, a->softcap, nullptr, nullptr, 0};
+    // Numbers whose products with log2 e or with one another would leave f32: a scale or a cap past 1e38 acts as 1e38 does (scores
+    // differ only where they pass it), and under a cap of less than 1e-30 of the scale every score but zero is the cap.
+    p.scale = std::fmax(-1e38f, std::fmin(1e38f, p.scale));
+    p.softcap = std::fmin(1e38f, p.softcap);
+    if (p.softcap > 0.f && std::fabs(p.scale) > 1e30f * p.softcap) p.scale = std::copysign(1e30f * p.softcap, p.scale);
     cudaStream_t s = (cudaStream_t)stream;
     const MaskedPlan plan = masked_plan(a);
     p.nsplit = plan.nsplit;

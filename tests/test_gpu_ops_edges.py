@@ -341,3 +341,23 @@ def test_the_calls_can_be_captured_in_a_graph(nq):
         want = layer()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert L.load().eg2_device_status() == 0
+
+
+# ---- scales and caps at the ends of 32 bits -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("nq", [3, 200])
+def test_caps_and_scales_at_the_ends_of_the_type(dtype, nh, nkv, hd, nq):
+    """A cap near the type's largest value caps nothing; one near its smallest leaves all scores equal; a score of zero is zero
+    under any scale."""
+    ql, kl = [nq], [333]
+    q, k, v = normal(91, nq, nh, hd, dtype=dtype), normal(92, 333, nkv, hd, dtype=dtype), normal(93, 333, nkv, hd, dtype=dtype)
+    scale = hd ** -0.5
+    for softcap in (1e30, 2.3e38, torch.finfo(F32).max):
+        check_attention(q, k, v, ql, kl, attend(q, k, v, ql, kl, scale=scale, softcap=softcap), scale=scale)
+    zero = q.clone()
+    zero[:, :, :] = 0.0
+    for opt in (dict(scale=torch.finfo(F32).max), dict(scale=-3e38), dict(scale=3e38, softcap=2.0), dict(scale=1.0, softcap=1e-40)):
+        check_attention(zero, k, v, ql, kl, attend(zero, k, v, ql, kl, **opt), scale=1.0)
+    # every score is within 1e-38 of zero, whatever its sign
+    got = attend(q, k, v, ql, kl, scale=scale, softcap=1e-40)
+    check_attention(zero, k, v, ql, kl, got, scale=1.0)
