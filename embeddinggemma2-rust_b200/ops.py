@@ -251,7 +251,7 @@ def quantize_rows(x):
 def _i8(t, name: str):
     if t.dim() != 2 or t.dtype != torch.int8 or (t.shape[1] > 1 and t.stride(1) != 1):
         _bad(f"{name}: expected int8 [rows, k] with contiguous rows, got {tuple(t.shape)} {t.dtype}")
-    ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
+    ld = t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16  # of one row it says nothing
     if ld % 16 or t.data_ptr() % 16 or ld < t.shape[1]:
         _bad(f"{name}: rows must start at multiples of 16 bytes (row stride {ld})")
     return ld

@@ -361,3 +361,15 @@ def test_caps_and_scales_at_the_ends_of_the_type(dtype, nh, nkv, hd, nq):
     # every score is within 1e-38 of zero, whatever its sign
     got = attend(q, k, v, ql, kl, scale=scale, softcap=1e-40)
     check_attention(zero, k, v, ql, kl, got, scale=1.0)
+
+
+def test_gemm_i8_of_one_row_from_a_buffer_of_any_stride():
+    buf = torch.randint(-127, 128, (8, 1000), dtype=torch.int8, generator=torch.Generator().manual_seed(94)).cuda()
+    w, ws = ops.quantize_rows(normal(95, 40, 777))
+    one = torch.ones(1, device="cuda")
+    for row in (0, 2, 4):  # 16-byte aligned
+        a = buf[row : row + 1, :777]
+        got = ops.gemm_i8(a, one, w, ws, out_dtype=F32)
+        want = (a.double() @ w.double().T) * ws.double()
+        assert bool(((got.double() - want).abs() <= 2.0**-22 * want.abs()).all())
+        assert torch.equal(ops.gemm_i8(w, ws, a, one, out_dtype=F32).T, got)
