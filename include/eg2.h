@@ -198,7 +198,7 @@ int eg2_rotary(int kind, int layout, int inverse, const void* q, int64_t ldq, in
  * softmax), -infinity is a mask. A query that sees no key gets out 0 and lse -inf; what hidden keys hold (NaN, infinities) does not
  * change a bit of any row. A row that sees a NaN, or an infinite value, ends NaN or infinite, however small the key's weight: a
  * channel of V with infinities of one sign in that infinity (or NaN, where the weight has vanished in f32).
- * hd up to 512. bf16 runs on the tensor cores when hd, the strides and the pointers are multiples of 8 elements. */
+ * scale and softcap past 1e38 act as 1e38. hd up to 512. bf16 runs on the tensor cores when hd, the strides and the pointers are multiples of 8 elements. */
 #define EG2_MASKED_MAX_LEN (1 << 20) /* tokens of one sequence */
 #define EG2_MASKED_MAX_RADIUS 1024
 typedef struct {
