@@ -860,7 +860,7 @@ __global__ void __launch_bounds__(AMT_THREADS, 1)
         const bool raw = !(p.softcap > 0.f) && !p.slopes && !p.table && a > 0.f;
         const float sc = raw ? a : 1.f;
         // cap2 tanh(a s) = s (c0 + c1 s^2 + ...) where |a s| <= 1/2, as long as the powers of a stay in range: of scale / softcap between
-        // 1e-4 and 1e3, and |score| <= softcap / 2. A warp's tile with a score past that is done twice, and so is every tile outside
+        // 1e-4 and 1e3, and |score| <= softcap / 2. A warp's tile with a score past that, a hidden one too, is done twice, and so is every tile outside
         // that range of a: 8,192 tokens, scores of deviation 2 under a cap of 50 / of 5: 655 / 1,300 us (12 heads of 64), 485 / 900 (8 over 2
         // of 128), 352 / 560 (4 over 2 of 256), 1,062 / 1,478 (4 over 1 of 512).
         const bool near_ok = fabsf(a) > 1e-4f && fabsf(a) < 1e3f;
